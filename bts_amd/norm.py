@@ -1,0 +1,73 @@
+"""Layer normalisation with autograd on the HIP kernels `bts_layernorm_fwd` / `bts_layernorm_bwd`.
+
+The decoder normalises with BatchNorm (bts.py:155-172), whose statistics are taken over the images of ONE rank; layer normalisation does
+not depend on the batch.  ``LayerNorm`` takes the place of ``torch.nn.LayerNorm`` (same arguments, parameters and state-dict keys),
+``LayerNorm2d`` normalises the channels at every pixel of an NCHW map, where ``nn.BatchNorm2d`` would normalise the batch.
+
+Inputs are f32 or bf16, parameters and their gradients f32, statistics f32.  No second derivatives, no CPU path.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import ops
+from ._lib import BtsAmdError, require_gpu
+
+__all__ = ["layer_norm", "LayerNorm", "LayerNorm2d"]
+
+
+def _rows(t):
+    """t itself where the kernels can walk it (contiguous, evenly strided rows), else a dense copy."""
+    return t if ops.row_stride(t) is not None else t.contiguous()
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        x = _rows(x)
+        if not any(ctx.needs_input_grad):
+            return ops.layer_norm_fwd(x, weight, bias, eps)
+        y, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps, want_stats=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return ops.layer_norm_bwd(_rows(dy), x, mean, rstd, weight, need[0], need[1], need[2]) + (None,)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., C], 1 <= C <= 16384; weight and bias f32 [C] or None."""
+    require_gpu(x)
+    if x.dim() == 0:
+        raise BtsAmdError("layer_norm: x must have at least one axis")
+    return _LayerNormFn.apply(x, weight, bias, float(eps))
+
+
+class LayerNorm(nn.LayerNorm):
+    """``torch.nn.LayerNorm`` on the HIP kernels: normalises over the trailing axes `normalized_shape`."""
+
+    def forward(self, x):
+        shape = tuple(self.normalized_shape)
+        if tuple(x.shape[x.dim() - len(shape):]) != shape or x.dim() < len(shape):
+            raise BtsAmdError("LayerNorm over %s got an input of shape %s" % (shape, tuple(x.shape)))
+        if len(shape) == 1:
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        flat = (t if t is None else t.reshape(-1) for t in (self.weight, self.bias))
+        return layer_norm(x.flatten(x.dim() - len(shape)), *flat, self.eps).view(x.shape)
+
+
+class LayerNorm2d(nn.LayerNorm):
+    """Normalises the C channels at every pixel of x [N, C, H, W].  A channels-last map is read and written in place of its layout; a
+    contiguous NCHW map costs a copy, and the result is channels-last either way."""
+
+    def __init__(self, num_channels, eps=1e-5, elementwise_affine=True, **kw):
+        super().__init__(num_channels, eps=eps, elementwise_affine=elementwise_affine, **kw)
+
+    def forward(self, x):
+        if x.dim() != 4 or x.shape[1] != self.normalized_shape[0]:
+            raise BtsAmdError("LayerNorm2d over %d channels got an input of shape %s" % (self.normalized_shape[0], tuple(x.shape)))
+        return layer_norm(x.permute(0, 2, 3, 1), self.weight, self.bias, self.eps).permute(0, 3, 1, 2)

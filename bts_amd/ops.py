@@ -36,6 +36,24 @@ def pix_stride(t):
     return s
 
 
+class on_device:
+    """`with on_device(t):` -- launches and stream_ptr() go to t's device, whatever the caller's current one is."""
+
+    def __init__(self, t):
+        self.idx, self.was = t.device.index, -1
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.idx:
+            self.was = cur
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.was >= 0:
+            torch.cuda.set_device(self.was)
+        return False
+
+
 def npix(t):
     return t.shape[0] * t.shape[1] * t.shape[2]
 
@@ -447,6 +465,99 @@ def bn_bwd_multi(tensors, eps, relu, use_batch_stats, tag=None):
     if profiler.ACTIVE is not None:      # reduction: x + n dy; apply: x + n dy read, dx written (+ read when accumulating)
         profiler.note("bn_bwd_multi", "hbm", npix(x0) * x0.element_size() * passes, tag)
     call("bts_bn_bwd_multi", C.byref(d), _p(ws), stream_ptr())
+
+
+# ---------------------------------------------------------------------------------------------
+# layer normalisation over the last axis (csrc/layernorm.hip); autograd: bts_amd/norm.py
+# ---------------------------------------------------------------------------------------------
+LN_MAX_C = 16384
+
+
+def row_stride(t):
+    """(rows, row stride in elements) of a tensor [..., C] whose last axis is contiguous and whose rows are evenly strided -- a channel
+    slice of a wider buffer is one --, else None."""
+    if t.dim() == 0 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        return None
+    if t.numel() == 0:
+        return 0, t.shape[-1]
+    rows, stride = 1, None
+    for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if stride is None:
+            stride = st
+        elif st != rows * stride:
+            return None
+        rows *= n
+    return rows, t.shape[-1] if stride is None else stride
+
+
+def _ln_rows(t, what, like=None):
+    _lib.require_gpu(t)
+    rs = row_stride(t)
+    if rs is None:
+        raise BtsAmdError("%s: rows must be contiguous and evenly strided, got %s with strides %s" % (what, tuple(t.shape), t.stride()))
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise BtsAmdError("%s: %s %s on %s does not match x: %s %s on %s" % (what, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
+    if not 1 <= t.shape[-1] <= LN_MAX_C:
+        raise BtsAmdError("%s: the normalised axis must have 1..%d elements, got %d" % (what, LN_MAX_C, t.shape[-1]))
+    return rs
+
+
+def _ln_vec(t, n, x, what):
+    """An f32 vector of n elements on x's device (or None)."""
+    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != x.device):
+        raise BtsAmdError("%s must be a contiguous f32 tensor of %d elements on %s, got %s %s on %s" % (what, n, x.device, tuple(t.shape), t.dtype, t.device))
+    return t
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=False):
+    """x [..., C] f32 / bf16 (rows evenly strided) -> y = (x - mean) / sqrt(var + eps) * weight + bias, dense, in x's dtype; with
+    want_stats also (mean, rstd), f32 [rows]: what layer_norm_bwd takes."""
+    M, xs = _ln_rows(x, "layer_norm_fwd")
+    Cc = x.shape[-1]
+    _ln_vec(weight, Cc, x, "layer_norm_fwd: weight")
+    _ln_vec(bias, Cc, x, "layer_norm_fwd: bias")
+    if not eps >= 0.0:
+        raise BtsAmdError("layer_norm_fwd: eps must be >= 0, got %r" % (eps,))
+    dt = dtype_code(x.dtype)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if want_stats else None
+    if M:
+        if profiler.ACTIVE is not None:
+            profiler.note("layernorm_fwd", "hbm", 2 * M * Cc * x.element_size())
+        with on_device(x):
+            call("bts_layernorm_fwd", _p(x), dt, xs, _p(y), Cc, M, Cc, _p(weight), _p(bias), float(eps), _p(stats[0] if want_stats else None),
+                 _p(stats[1] if want_stats else None), stream_ptr())
+    return (y, stats[0], stats[1]) if want_stats else y
+
+
+def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dweight=True, want_dbias=True):
+    """Gradients (dx, dweight, dbias) of layer_norm_fwd; one that is not wanted is None.  dx is dense, in x's dtype; dweight and dbias are
+    f32 [C], sums over all rows in a fixed order."""
+    M, xs = _ln_rows(x, "layer_norm_bwd")
+    _, dys = _ln_rows(dy, "layer_norm_bwd: dy", x)
+    Cc = x.shape[-1]
+    _ln_vec(weight, Cc, x, "layer_norm_bwd: weight")
+    for t in (mean, rstd):
+        if t is None:
+            raise BtsAmdError("layer_norm_bwd needs mean and rstd (layer_norm_fwd with want_stats)")
+        _ln_vec(t, M, x, "layer_norm_bwd: mean / rstd")
+    dt = dtype_code(x.dtype)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+    make = torch.empty if M else torch.zeros
+    dw = make(Cc, dtype=torch.float32, device=x.device) if want_dweight else None
+    db = make(Cc, dtype=torch.float32, device=x.device) if want_dbias else None
+    if M and (want_dx or want_dweight or want_dbias):
+        with on_device(x):
+            ws = None
+            if want_dweight or want_dbias:
+                ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc) // 4, dtype=torch.float32, device=x.device)
+            if profiler.ACTIVE is not None:
+                profiler.note("layernorm_bwd", "hbm", M * Cc * x.element_size() * (3 if want_dx else 2))
+            call("bts_layernorm_bwd", _p(dy), dys, _p(x), xs, _p(dx), Cc, dt, M, Cc, _p(weight), _p(mean), _p(rstd), _p(dw), _p(db), _p(ws),
+                 stream_ptr())
+    return dx, dw, db
 
 
 def act_bwd(dy, y, act, out=None, out_dtype=None, out_channels=None, y_scale=1.0, y_scale_n=None, accumulate=False):

@@ -502,6 +502,22 @@ int bts_adamw_step(float* const* params, float* const* grads, float* const* exp_
  * checkpoint is written (bts_main.py:498-503). */
 int bts_adamw_advance(float* dev_hyper_rows, int n_groups, bts_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Layer normalisation over the last axis: M rows of C elements, contiguous inside a row, `*_stride` elements from row to row
+ * (0 for a row that repeats; outputs: >= C).  The batch-independent normalisation next to bts_bn_apply / bts_bn_bwd.
+ *     mu = mean(x), v = mean((x - mu)^2), r = 1 / sqrt(v + eps), y = (x - mu) r w + b
+ *     h = dy w, xh = (x - mu) r: dx = r (h - mean(h) - xh mean(h xh)), dw = sum dy xh, db = sum dy
+ * x, y, dy, dx are f32 or bf16 (`dtype`), everything else is f32.  w == NULL: 1, b == NULL: 0.  mean / rstd [M]: both, or both
+ * NULL (forward: not wanted; backward: required).  dx, dw, db: any that is not wanted is NULL, at least one is not.
+ * Pointers need the alignment of their element only.  Outputs must not overlap inputs.  C <= 16384 (BTS_ERR_UNSUPPORTED above).
+ * The backward pass takes a workspace of bts_layernorm_bwd_workspace_bytes (not for dx alone); its sums have a fixed order.
+ * ---------------------------------------------------------------------------------- */
+int bts_layernorm_fwd(const void* x, int dtype, long x_stride, void* y, long y_stride, long M, int C, const float* w, const float* b,
+                      float eps, float* mean, float* rstd, bts_stream_t stream);
+long bts_layernorm_bwd_workspace_bytes(int dtype, long M, int C);
+int bts_layernorm_bwd(const void* dy, long dy_stride, const void* x, long x_stride, void* dx, long dx_stride, int dtype, long M, int C,
+                      const float* w, const float* mean, const float* rstd, float* dw, float* db, void* workspace, bts_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,57 @@
+"""Host side of the layer normalisation: layouts, refusals of the wrappers and of the C entries (no GPU needed: every refused call
+returns before a launch)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from bts_amd import _lib, ops
+from bts_amd.norm import LayerNorm, LayerNorm2d, layer_norm
+
+
+def test_row_stride():
+    t = torch.empty(4, 5, 6)
+    assert ops.row_stride(t) == (20, 6)
+    assert ops.row_stride(t[:, :, 1:4]) == (20, 6)
+    assert ops.row_stride(t[:, 1:3]) is None                       # rows in groups
+    assert ops.row_stride(t[1:2, 1:3]) == (2, 6)
+    assert ops.row_stride(t.transpose(1, 2)) is None               # last axis not contiguous
+    assert ops.row_stride(t[0, 0]) == (1, 6)
+    assert ops.row_stride(t[..., :1]) == (20, 6)
+    assert ops.row_stride(t[::2, :1]) == (2, 60)
+    assert ops.row_stride(torch.empty(1, 6).expand(5, 6)) == (5, 0)
+    assert ops.row_stride(torch.empty(1, 3, 6).expand(5, 3, 6)) is None
+    assert ops.row_stride(torch.empty(0, 6)) == (0, 6)
+    assert ops.row_stride(torch.empty(())) is None
+    assert ops.row_stride(torch.empty(2, 8, 3, 5).contiguous(memory_format=torch.channels_last).permute(0, 2, 3, 1)) == (30, 8)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(3, 8)
+    for call in (lambda: layer_norm(x), lambda: LayerNorm(8)(x), lambda: LayerNorm2d(8)(torch.randn(1, 8, 2, 2)), lambda: ops.layer_norm_fwd(x)):
+        with pytest.raises(_lib.BtsAmdError):
+            call()
+
+
+def test_c_entries_refuse_bad_arguments():
+    lib, p, n = _lib.load(), C.c_void_p(4096), C.c_void_p(0)        # 4096: never read, the calls below end before any launch
+    good = dict(x=p, dtype=0, xs=8, y=C.c_void_p(8192), ys=8, M=4, C=8, w=n, b=n, eps=1e-5, mean=n, rstd=n, st=n)
+    fwd = lambda **k: lib.bts_layernorm_fwd(*{**good, **k}.values())   # noqa: E731
+    for bad in (dict(x=n), dict(y=n), dict(y=p), dict(dtype=2), dict(dtype=-1), dict(M=0), dict(M=-3), dict(C=0), dict(xs=-1), dict(ys=7), dict(eps=-1.0),
+                dict(eps=float("nan")), dict(mean=p), dict(rstd=p), dict(x=C.c_void_p(4098)), dict(y=C.c_void_p(8193), dtype=1)):
+        assert fwd(**bad) == -1, bad
+    assert fwd(C=16385, xs=16385, ys=16385) == -3
+    good_b = dict(dy=p, dys=8, x=C.c_void_p(8192), xs=8, dx=C.c_void_p(16384), dxs=8, dtype=0, M=4, C=8, w=n, mean=p, rstd=p, dw=p, db=p, ws=p, st=n)
+    bwd = lambda **k: lib.bts_layernorm_bwd(*{**good_b, **k}.values())   # noqa: E731
+    for bad in (dict(dy=n), dict(x=n), dict(mean=n), dict(rstd=n), dict(ws=n), dict(ws=C.c_void_p(4097)), dict(dx=p), dict(dx=C.c_void_p(8192)), dict(dxs=7),
+                dict(dtype=3), dict(M=0), dict(C=0), dict(dys=-8), dict(dx=n, dw=n, db=n)):
+        assert bwd(**bad) == -1, bad
+    assert bwd(C=16385, xs=16385, dys=16385, dxs=16385) == -3
+    size = lib.bts_layernorm_bwd_workspace_bytes
+    assert size(0, 10, 16385) == size(0, 0, 8) == size(2, 10, 8) == 0
+    assert size(0, 1, 8) == 64 and size(1, 10 ** 9, 96) >= size(1, 10, 96) > 0
+
+
+def test_modules_have_torch_parameters():
+    assert [(k, tuple(v.shape)) for k, v in LayerNorm(12).state_dict().items()] == [(k, tuple(v.shape)) for k, v in torch.nn.LayerNorm(12).state_dict().items()]
+    assert list(LayerNorm2d(12, bias=False).state_dict()) == ["weight"] and list(LayerNorm2d(12, elementwise_affine=False).state_dict()) == []
