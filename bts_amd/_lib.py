@@ -10,6 +10,8 @@ import os
 
 import torch  # noqa: F401  (must be imported before the dlopen below)
 
+from . import profiler
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libbts_amd.so")
 
@@ -187,29 +189,41 @@ def load():
     return lib
 
 
+_entries = {}
+
+
 def call(name, *args):
     """Invoke an entry point and raise on a non-zero status."""
-    from . import profiler
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
     if profiler.ACTIVE is not None and name not in _NO_CHECK:
         note = profiler.take() or (name[4:], "hbm", 0.0, None, 0.0)      # undescribed launches are still timed (zero work)
         s, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         s.record()
-        rc = getattr(load(), name)(*args)
+        rc = fn(*args)
         e.record()
         if rc != ERR_UNSUPPORTED:      # nothing was launched: the caller retries with other launches, which record their own work
             profiler.ACTIVE.add(note[0], note[1], note[2], s, e, note[3], note[4])
-        if rc != 0:
-            raise BtsAmdError("%s failed: %s (%d)" % (name, ERRORS.get(rc, "?"), rc), rc)
-        return rc
-    rc = getattr(load(), name)(*args)
-    if name not in _NO_CHECK and rc != 0:
+    else:
+        rc = fn(*args)
+    if rc != 0 and name not in _NO_CHECK:
         raise BtsAmdError("%s failed: %s (%d)" % (name, ERRORS.get(rc, "?"), rc), rc)
     return rc
 
 
+current_device = torch._C._cuda_getDevice               # of the calling thread; only reached once a HIP tensor exists
+
+
+def raw_stream():
+    """The current PyTorch HIP stream of the current device as an integer (what ctypes takes for a void*).  Asked of the runtime binding
+    directly: building the Stream object costs ten times the call."""
+    return torch._C._cuda_getCurrentRawStream(current_device())
+
+
 def stream_ptr():
     """The current PyTorch HIP stream as a raw hipStream_t."""
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(raw_stream())
 
 
 def dtype_code(dt):

@@ -15,58 +15,92 @@ constexpr int kThreads = 256;       // rows of up to 64 lanes: 256 / LANES rows 
 // at any alignment), so one kernel serves every width, stride and storage offset
 typedef uint32_t u32x4_a2_t __attribute__((ext_vector_type(4), aligned(2)));
 
-template <typename T>
+// ODD: C is no multiple of the vector, so a row's last vector is taken element by element
+template <typename T, bool ODD>
 __device__ __forceinline__ void load_vec(const void* base, long off, int c0, int C, float* f) {
     const typename T::elem_t* p = (const typename T::elem_t*)base + off + c0;
-    if (c0 + T::kVec <= C) {
+    if (ODD ? c0 + T::kVec <= C : c0 < C) {
         const u32x4_a2_t u = *(const u32x4_a2_t*)p;
         const u32x4_t v = {u.x, u.y, u.z, u.w};
         T::unpack(v, f);
     } else {
 #pragma unroll
-        for (int e = 0; e < T::kVec; ++e) f[e] = c0 + e < C ? T::ld(p, e) : 0.f;
+        for (int e = 0; e < T::kVec; ++e) f[e] = ODD && c0 + e < C ? T::ld(p, e) : 0.f;
     }
 }
-template <typename T>
+template <typename T, bool ODD>
 __device__ __forceinline__ void store_vec(void* base, long off, int c0, int C, const float* f) {
     typename T::elem_t* p = (typename T::elem_t*)base + off + c0;
-    if (c0 + T::kVec <= C) {
+    if (ODD ? c0 + T::kVec <= C : c0 < C) {
         const u32x4_t v = T::pack(f);
         *(u32x4_a2_t*)p = (u32x4_a2_t){v.x, v.y, v.z, v.w};
-    } else {
+    } else if (ODD) {
 #pragma unroll
         for (int e = 0; e < T::kVec; ++e)
             if (c0 + e < C) T::st(p, e, f[e]);
     }
 }
-// per-channel f32 parameters of one vector; absent channels take `fill`
-template <int V>
+// per-channel f32 parameters of one vector (V = 4 or 8); absent parameters take `fill`
+template <int V, bool ODD>
 __device__ __forceinline__ void load_param(const float* w, int c0, int C, float fill, float* f) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = w && c0 + e < C ? w[c0 + e] : fill;
-}
-
-// Sum over the LANES lanes that hold a row.  LANES > 64: the whole block, through LDS (`red`: one float per wave, two sets used in
-// turn so that one barrier per sum is enough).
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-    if constexpr (LANES <= 64) {
+    for (int e = 0; e < V; ++e) f[e] = fill;
+    if (w) {
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-        return v;
-    } else {
-        constexpr int W = LANES / 64;
-        v = wave_sum(v);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) s += red[i];
-        return s;
+        for (int i = 0; i < V; i += 4) load_vec<F32, ODD>(w, 0, c0 + i, C, f + i);
     }
 }
 
-template <typename T, int LANES, int K>
+template <typename T, bool ODD>
+__device__ __forceinline__ void store_sums(float* base, int c0, int C, const float* f) {
+#pragma unroll
+    for (int i = 0; i < T::kVec; i += 4) store_vec<F32, ODD>(base, 0, c0 + i, C, f + i);
+}
+
+// v + the value that another lane of the row holds: lanes 1, 2 (quad), then mirrored halves of 8 and 16, then 16 and 32 lanes away by
+// the permlane swaps.  Every step leaves equal sums in all lanes that took part, so "mirrored" pairs the same sums as "exchanged",
+// and no step goes through the LDS pipe (ds_bpermute, what __shfl_xor makes, costs its latency six times a sum).
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float add_lane16(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_lane32(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// sum over aligned groups of N lanes (N a power of two, at most the wave)
+template <int N>
+__device__ __forceinline__ float lane_sum(float v) {
+    if constexpr (N >= 2) v = add_dpp<0xB1>(v);        // quad_perm 1,0,3,2
+    if constexpr (N >= 4) v = add_dpp<0x4E>(v);        // quad_perm 2,3,0,1
+    if constexpr (N >= 8) v = add_dpp<0x141>(v);       // row_half_mirror
+    if constexpr (N >= 16) v = add_dpp<0x140>(v);      // row_mirror
+    if constexpr (N >= 32) v = add_lane16(v);
+    if constexpr (N >= 64) v = add_lane32(v);
+    return v;
+}
+
+// Sum over the LANES lanes that hold a row.  LANES > 64: the whole block, through LDS (`red`: one float per wave).  Two sums of one
+// row use two sets, so one barrier per sum is enough: a set is written again only behind the barrier of the other.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+    v = lane_sum<LANES < 64 ? LANES : 64>(v);
+    if constexpr (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[threadIdx.x & (LANES / 64 - 1)];
+        v = lane_sum<LANES / 64>(v);
+    }
+    return v;
+}
+
+template <typename T, int LANES, int K, bool ODD>
 __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(const void* __restrict__ x, long xs, void* __restrict__ y, long ys,
                                                                                long M, int C, const float* __restrict__ w,
                                                                                const float* __restrict__ b, float eps,
@@ -77,8 +111,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(c
     float wv[K][V], bv[K][V];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        load_param<V>(w, (lane + j * LANES) * V, C, 1.f, wv[j]);
-        load_param<V>(b, (lane + j * LANES) * V, C, 0.f, bv[j]);
+        load_param<V, ODD>(w, (lane + j * LANES) * V, C, 1.f, wv[j]);
+        load_param<V, ODD>(b, (lane + j * LANES) * V, C, 0.f, bv[j]);
     }
     const float inv = 1.f / (float)C;
     for (long r0 = (long)blockIdx.x * RPB; r0 < M; r0 += (long)gridDim.x * RPB) {
@@ -88,7 +122,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(c
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const int c0 = (lane + j * LANES) * V;
-            load_vec<T>(x, on ? row * xs : 0, c0, on ? C : 0, f[j]);
+            load_vec<T, ODD>(x, on ? row * xs : 0, c0, on ? C : 0, f[j]);
 #pragma unroll
             for (int e = 0; e < V; ++e) s += f[j][e];
         }
@@ -111,31 +145,30 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(c
             float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = f[j][e] * rs * wv[j][e] + bv[j][e];
-            store_vec<T>(y, on ? row * ys : 0, (lane + j * LANES) * V, on ? C : 0, o);
+            store_vec<T, ODD>(y, on ? row * ys : 0, (lane + j * LANES) * V, on ? C : 0, o);
         }
     }
 }
 
 // Every block walks rows in steps of the grid and keeps the sums of dy xh and dy over its rows in registers; it writes one partial row
 // [2][C] (ws), ln_bwd_final_kernel adds the rows in a fixed order: no atomics, the gradients of the parameters are reproducible.
-template <typename T, int LANES, int K, bool PARAM>
+template <typename T, int LANES, int K, bool ODD, bool PARAM>
 __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(const void* __restrict__ dy, long dys, const void* __restrict__ x, long xs,
                                                                                void* __restrict__ dx, long dxs, long M, int C,
                                                                                const float* __restrict__ w, const float* __restrict__ mean,
                                                                                const float* __restrict__ rstd, float* __restrict__ ws) {
     constexpr int V = T::kVec, RPB = LANES > 64 ? 1 : kThreads / LANES;
-    __shared__ float red[2][2][LANES > 64 ? LANES / 64 : 1];
+    __shared__ float red[2][LANES > 64 ? LANES / 64 : 1];
     const int lane = threadIdx.x % LANES;
     float wv[K][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        load_param<V>(w, (lane + j * LANES) * V, C, 1.f, wv[j]);
+        load_param<V, ODD>(w, (lane + j * LANES) * V, C, 1.f, wv[j]);
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[j][e] = db[j][e] = 0.f;
     }
     const float inv = 1.f / (float)C;
-    int turn = 0;
-    for (long r0 = (long)blockIdx.x * RPB; r0 < M; r0 += (long)gridDim.x * RPB, turn ^= 1) {
+    for (long r0 = (long)blockIdx.x * RPB; r0 < M; r0 += (long)gridDim.x * RPB) {
         const long row = r0 + threadIdx.x / LANES;
         const bool on = row < M;
         const float mu = on ? mean[row] : 0.f, rs = on ? rstd[row] : 0.f;
@@ -143,8 +176,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(c
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const int c0 = (lane + j * LANES) * V;
-            load_vec<T>(x, on ? row * xs : 0, c0, on ? C : 0, f[j]);
-            load_vec<T>(dy, on ? row * dys : 0, c0, on ? C : 0, g[j]);
+            load_vec<T, ODD>(x, on ? row * xs : 0, c0, on ? C : 0, f[j]);
+            load_vec<T, ODD>(dy, on ? row * dys : 0, c0, on ? C : 0, g[j]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 f[j][e] = on && c0 + e < C ? (f[j][e] - mu) * rs : 0.f;
@@ -158,78 +191,66 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(c
             }
         }
         if (dx) {
-            const float m1 = row_sum<LANES>(s1, red[turn][0]) * inv, m2 = row_sum<LANES>(s2, red[turn][1]) * inv;
+            const float m1 = row_sum<LANES>(s1, red[0]) * inv, m2 = row_sum<LANES>(s2, red[1]) * inv;
 #pragma unroll
             for (int j = 0; j < K; ++j) {
                 float o[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) o[e] = rs * (g[j][e] * wv[j][e] - m1 - f[j][e] * m2);
-                store_vec<T>(dx, on ? row * dxs : 0, (lane + j * LANES) * V, on ? C : 0, o);
+                store_vec<T, ODD>(dx, on ? row * dxs : 0, (lane + j * LANES) * V, on ? C : 0, o);
             }
         }
     }
     if constexpr (PARAM) {
         float* out = ws + (long)blockIdx.x * 2 * C;
-        if constexpr (LANES >= 256) {
+        if constexpr (RPB == 1) {
 #pragma unroll
-            for (int j = 0; j < K; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const int c = (lane + j * LANES) * V + e;
-                    if (c < C) {
-                        out[c] = dw[j][e];
-                        out[C + c] = db[j][e];
-                    }
-                }
+            for (int j = 0; j < K; ++j) {
+                store_sums<T, ODD>(out, (lane + j * LANES) * V, C, dw[j]);
+                store_sums<T, ODD>(out + C, (lane + j * LANES) * V, C, db[j]);
+            }
         } else {
-            // the block's kThreads / LANES rows: within a wave by exchange, across its four waves through LDS
-            __shared__ float part[kThreads / 64][2][LANES * K * V];
+            // the block's RPB rows of sums, through LDS: first dw, then db
+            constexpr int W = LANES * K * V;
+            __shared__ float part[RPB * W];
 #pragma unroll
-            for (int j = 0; j < K; ++j)
+            for (int t = 0; t < 2; ++t) {
+                if (t) __syncthreads();
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float a = dw[j][e], c = db[j][e];
+                for (int j = 0; j < K; ++j)
 #pragma unroll
-                    for (int o = LANES; o < 64; o <<= 1) {
-                        a += __shfl_xor(a, o, 64);
-                        c += __shfl_xor(c, o, 64);
-                    }
-                    if ((int)(threadIdx.x & 63) < LANES) {
-                        part[threadIdx.x >> 6][0][(lane + j * LANES) * V + e] = a;
-                        part[threadIdx.x >> 6][1][(lane + j * LANES) * V + e] = c;
-                    }
+                    for (int e = 0; e < V; ++e) part[(threadIdx.x / LANES) * W + (lane + j * LANES) * V + e] = t ? db[j][e] : dw[j][e];
+                __syncthreads();
+                for (int c = threadIdx.x; c < C; c += kThreads) {
+                    float a = 0.f;
+#pragma unroll 8
+                    for (int i = 0; i < RPB; ++i) a += part[i * W + c];
+                    out[(long)t * C + c] = a;
                 }
-            __syncthreads();
-            for (int c = threadIdx.x; c < C; c += kThreads) {
-                float a = 0.f, d = 0.f;
-#pragma unroll
-                for (int i = 0; i < kThreads / 64; ++i) {
-                    a += part[i][0][c];
-                    d += part[i][1][c];
-                }
-                out[c] = a;
-                out[C + c] = d;
             }
         }
     }
 }
 
-// ws [rows][2][C] -> dw, db: 16 columns of the 2 C x 16 row lanes per block, combined in a fixed order
-__global__ __launch_bounds__(256) void ln_bwd_final_kernel(const float* __restrict__ ws, int rows, int C, float* __restrict__ dw, float* __restrict__ db) {
-    __shared__ float part[16][17];
+// ws [rows][2][C] -> dw, db: 16 of the 2 C columns x 64 row lanes per block, combined in a fixed order
+__global__ __launch_bounds__(1024) void ln_bwd_final_kernel(const float* __restrict__ ws, int rows, int C, float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ float part[64][17];
     const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
     const long c = (long)blockIdx.x * 16 + cl, n = 2l * C;
     float s = 0.f;
-    if (c < n)
-        for (int r = rl; r < rows; r += 16) s += ws[r * n + c];
+    if (c < n) {
+#pragma unroll 8
+        for (int r = rl; r < rows; r += 64) s += ws[r * n + c];
+    }
     part[rl][cl] = s;
     __syncthreads();
-    if (rl == 0 && c < n) {
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) t += part[i][cl];
-        if (c < C) { if (dw) dw[c] = t; }
-        else if (db) db[c - C] = t;
+    // 16 waves: wave i adds the 64 sums of column i
+    const int col = threadIdx.x >> 6;
+    const float t = lane_sum<64>(part[threadIdx.x & 63][col]);
+    const long cc = (long)blockIdx.x * 16 + col;
+    if ((threadIdx.x & 63) == 0 && cc < n) {
+        if (cc < C) { if (dw) dw[cc] = t; }
+        else if (db) db[cc - C] = t;
     }
 }
 
@@ -240,19 +261,31 @@ struct LnPlan {
 
 constexpr int kLnMaxC = 16384;
 
-// lanes (a power of four) and vectors per lane (<= kmax): the fewest lanes that hold a row
-static LnPlan ln_plan(int V, long M, int C, int kmax, int per_cu) {
+// Lanes of a row and vectors per lane.  A row of up to 64 vectors takes one vector per lane: neighbouring lanes read neighbouring 16
+// bytes and several rows share a wave.  Up to 64 lanes x 16 elements stay in one wave (no barrier), longer rows take a block at 8
+// elements per lane, and 16 above 8192 elements.  Both sides, forward / backward with its sums, us: 856064 x 96 bf16 16 x 1: 70 / 106,
+// 8 x 2: 71 / 102, 4 x 3: 95 / 166; 400000 x 32 f32 8 x 1: 20.3 / 32.6, 2 x 4: 26.3 / 44.5; 13376 x 512 bf16 64 x 1: 7.3 / 15.8,
+// 16 x 4: 34 / 59; 16384 x 1024 bf16 64 x 2: 14.8 / 27.7, 128 x 1: 15.7 / 32.9; 8192 x 4096 bf16 512 x 1: 28.3 / 52, 256 x 2: 31.6 / 58.
+static void ln_lanes(int V, int C, int& lanes, int& k) {
     const int nv = (C + V - 1) / V;
+    int kmax = 1;
+    if (nv > 64) kmax = C <= 1024 ? 16 / V : (C <= 8192 ? 8 / V : 16 / V);
+    lanes = 1;
+    while (lanes * kmax < nv) lanes *= 2;
+    if (nv > 64 && C <= 1024) lanes = 64;
+    else if (nv > 64 && lanes < 256) lanes = 256;
+    k = (nv + lanes - 1) / lanes;
+}
+static LnPlan ln_plan(int dtype, long M, int C, int threads_per_cu) {
     LnPlan p;
-    p.lanes = 1;
-    while (p.lanes * kmax < nv) p.lanes *= 4;
-    p.k = (nv + p.lanes - 1) / p.lanes;
-    const int rpb = p.lanes > 64 ? 1 : kThreads / p.lanes;
-    const long want = (M + rpb - 1) / rpb, cap = (long)bts_cu_count() * per_cu;
+    ln_lanes(dtype == BTS_F32 ? 4 : 8, C, p.lanes, p.k);
+    const int threads = p.lanes > 64 ? p.lanes : kThreads;
+    const long want = (M + threads / p.lanes - 1) / (threads / p.lanes), cap = (long)bts_cu_count() * (threads_per_cu / threads);
     p.blocks = want < cap ? want : cap;
     return p;
 }
-static LnPlan ln_bwd_plan(int dtype, long M, int C) { return ln_plan(dtype == BTS_F32 ? 4 : 8, M, C, 4, C > 1024 ? 2 : 4); }
+static LnPlan ln_fwd_plan(int dtype, long M, int C) { return ln_plan(dtype, M, C, 2048); }
+static LnPlan ln_bwd_plan(int dtype, long M, int C) { return ln_plan(dtype, M, C, 1024); }
 
 static bool ln_args(const void* x, int dtype, long M, int C) {
     return x && (dtype == BTS_F32 || dtype == BTS_BF16) && M > 0 && C > 0 && ((uintptr_t)x & (dtype == BTS_F32 ? 3 : 1)) == 0;
@@ -260,21 +293,29 @@ static bool ln_args(const void* x, int dtype, long M, int C) {
 
 }  // namespace
 
-#define LN_K(T, L, F)               \
-    switch (p.k) {                  \
-        case 1: F(T, L, 1); break;  \
-        case 2: F(T, L, 2); break;  \
-        case 3: F(T, L, 3); break;  \
-        default: F(T, L, 4); break; \
+#define LN_ODD(T, L, K, F) \
+    if (C % T::kVec) { F(T, L, K, true); } else { F(T, L, K, false); }
+#define LN_K2(T, L, F) \
+    if (p.k == 1) { LN_ODD(T, L, 1, F) } else { LN_ODD(T, L, 2, F) }
+#define LN_K4(T, L, F)                                         \
+    switch (p.k) {                                             \
+        case 1: LN_ODD(T, L, 1, F) break;                      \
+        case 2: LN_ODD(T, L, 2, F) break;                      \
+        case 3: LN_ODD(T, L, (T::kVec == 4 ? 3 : 2), F) break; \
+        default: LN_ODD(T, L, (T::kVec == 4 ? 4 : 2), F)       \
     }
-#define LN_LANES(T, F)                       \
-    switch (p.lanes) {                       \
-        case 1: LN_K(T, 1, F) break;         \
-        case 4: LN_K(T, 4, F) break;         \
-        case 16: LN_K(T, 16, F) break;       \
-        case 64: LN_K(T, 64, F) break;       \
-        case 256: LN_K(T, 256, F) break;     \
-        default: LN_K(T, 1024, F) break;     \
+#define LN_LANES(T, F)                      \
+    switch (p.lanes) {                      \
+        case 1: LN_ODD(T, 1, 1, F) break;   \
+        case 2: LN_ODD(T, 2, 1, F) break;   \
+        case 4: LN_ODD(T, 4, 1, F) break;   \
+        case 8: LN_ODD(T, 8, 1, F) break;   \
+        case 16: LN_ODD(T, 16, 1, F) break; \
+        case 32: LN_ODD(T, 32, 1, F) break; \
+        case 64: LN_K4(T, 64, F) break;     \
+        case 256: LN_K2(T, 256, F) break;   \
+        case 512: LN_K2(T, 512, F) break;   \
+        default: LN_K4(T, 1024, F)          \
     }
 
 extern "C" int bts_layernorm_fwd(const void* x, int dtype, long x_stride, void* y, long y_stride, long M, int C, const float* w, const float* b,
@@ -282,10 +323,10 @@ extern "C" int bts_layernorm_fwd(const void* x, int dtype, long x_stride, void* 
     BTS_CHECK_ARG(ln_args(x, dtype, M, C) && y && y != x && x_stride >= 0 && y_stride >= C && !mean == !rstd && eps >= 0.f);
     BTS_CHECK_ARG(((uintptr_t)y & (dtype == BTS_F32 ? 3 : 1)) == 0);
     if (C > kLnMaxC) return BTS_ERR_UNSUPPORTED;
-    const LnPlan p = ln_plan(dtype == BTS_F32 ? 4 : 8, M, C, 4, 8);
+    const LnPlan p = ln_fwd_plan(dtype, M, C);
     hipStream_t st = (hipStream_t)stream;
-#define L_(T, LANES, K)                                                                                                              \
-    hipLaunchKernelGGL((ln_fwd_kernel<T, LANES, K>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, x, x_stride, y, \
+#define L_(T, LANES, K, ODD)                                                                                                                 \
+    hipLaunchKernelGGL((ln_fwd_kernel<T, LANES, K, ODD>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, x, x_stride, y, \
                        y_stride, M, C, w, b, eps, mean, rstd)
     if (dtype == BTS_F32) { LN_LANES(F32, L_) } else { LN_LANES(BF16, L_) }
 #undef L_
@@ -308,16 +349,16 @@ extern "C" int bts_layernorm_bwd(const void* dy, long dy_stride, const void* x, 
     const LnPlan p = ln_bwd_plan(dtype, M, C);
     hipStream_t st = (hipStream_t)stream;
     float* ws = (float*)workspace;
-#define L_(T, LANES, K)                                                                                                                        \
-    if (dw || db)                                                                                                                              \
-        hipLaunchKernelGGL((ln_bwd_kernel<T, LANES, K, true>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, dy, dy_stride, \
-                           x, x_stride, dx, dx_stride, M, C, w, mean, rstd, ws);                                                             \
-    else                                                                                                                                       \
-        hipLaunchKernelGGL((ln_bwd_kernel<T, LANES, K, false>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, dy,        \
-                           dy_stride, x, x_stride, dx, dx_stride, M, C, w, mean, rstd, ws)
+#define L_(T, LANES, K, ODD)                                                                                                         \
+    if (dw || db)                                                                                                                    \
+        hipLaunchKernelGGL((ln_bwd_kernel<T, LANES, K, ODD, true>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, \
+                           dy, dy_stride, x, x_stride, dx, dx_stride, M, C, w, mean, rstd, ws);                                      \
+    else                                                                                                                             \
+        hipLaunchKernelGGL((ln_bwd_kernel<T, LANES, K, ODD, false>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, \
+                           dy, dy_stride, x, x_stride, dx, dx_stride, M, C, w, mean, rstd, ws)
     if (dtype == BTS_F32) { LN_LANES(F32, L_) } else { LN_LANES(BF16, L_) }
 #undef L_
-    if (dw || db) hipLaunchKernelGGL(ln_bwd_final_kernel, dim3(ceil_div(2l * C, 16)), dim3(256), 0, st, ws, (int)p.blocks, C, dw, db);
+    if (dw || db) hipLaunchKernelGGL(ln_bwd_final_kernel, dim3(ceil_div(2l * C, 16)), dim3(1024), 0, st, ws, (int)p.blocks, C, dw, db);
     BTS_LAUNCH_CHECK();
     return BTS_OK;
 }

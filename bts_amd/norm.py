@@ -11,7 +11,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from ._lib import BtsAmdError, require_gpu
+from ._lib import BtsAmdError
 
 __all__ = ["layer_norm", "LayerNorm", "LayerNorm2d"]
 
@@ -25,26 +25,25 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         x = _rows(x)
-        if not any(ctx.needs_input_grad):
-            return ops.layer_norm_fwd(x, weight, bias, eps)
-        y, mean, rstd = ops.layer_norm_fwd(x, weight, bias, eps, want_stats=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = ops.layer_norm_fwd(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return ops.layer_norm_bwd(_rows(dy), x, mean, rstd, weight, need[0], need[1], need[2]) + (None,)
+        return (*ops.layer_norm_bwd(_rows(dy), x, stats, weight, need[0], need[1], need[2]), None)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., C], 1 <= C <= 16384; weight and bias f32 [C] or None."""
-    require_gpu(x)
     if x.dim() == 0:
         raise BtsAmdError("layer_norm: x must have at least one axis")
-    return _LayerNormFn.apply(x, weight, bias, float(eps))
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _LayerNormFn.apply(x, weight, bias, float(eps))
+    return ops.layer_norm_fwd(_rows(x), weight, bias, float(eps))
 
 
 class LayerNorm(nn.LayerNorm):

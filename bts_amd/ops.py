@@ -10,7 +10,7 @@ import ctypes as C
 import torch
 
 from . import _lib, profiler
-from ._lib import ACT_ELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, BtsAmdError, call, dtype_code, stream_ptr  # noqa: F401
+from ._lib import ACT_ELU, ACT_NONE, ACT_RELU, ACT_SIGMOID, BtsAmdError, call, current_device, dtype_code, raw_stream, stream_ptr  # noqa: F401
 
 
 def vec_of(dtype):
@@ -34,24 +34,6 @@ def pix_stride(t):
     if (H > 1 and t.stride(1) != W * s) or (N > 1 and t.stride(0) != H * W * s):
         raise BtsAmdError("NHWC tensor pixels are not evenly strided: %s %s" % (t.shape, t.stride()))
     return s
-
-
-class on_device:
-    """`with on_device(t):` -- launches and stream_ptr() go to t's device, whatever the caller's current one is."""
-
-    def __init__(self, t):
-        self.idx, self.was = t.device.index, -1
-
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.idx:
-            self.was = cur
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *exc):
-        if self.was >= 0:
-            torch.cuda.set_device(self.was)
-        return False
 
 
 def npix(t):
@@ -476,10 +458,13 @@ LN_MAX_C = 16384
 def row_stride(t):
     """(rows, row stride in elements) of a tensor [..., C] whose last axis is contiguous and whose rows are evenly strided -- a channel
     slice of a wider buffer is one --, else None."""
-    if t.dim() == 0 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dim() == 0:
         return None
-    if t.numel() == 0:
-        return 0, t.shape[-1]
+    Cc = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // Cc if Cc else 0, Cc
+    if Cc > 1 and t.stride(-1) != 1:
+        return None
     rows, stride = 1, None
     for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if n == 1:
@@ -489,74 +474,82 @@ def row_stride(t):
         elif st != rows * stride:
             return None
         rows *= n
-    return rows, t.shape[-1] if stride is None else stride
+    return rows, Cc if stride is None else stride
 
 
 def _ln_rows(t, what, like=None):
-    _lib.require_gpu(t)
     rs = row_stride(t)
     if rs is None:
         raise BtsAmdError("%s: rows must be contiguous and evenly strided, got %s with strides %s" % (what, tuple(t.shape), t.stride()))
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device()):
         raise BtsAmdError("%s: %s %s on %s does not match x: %s %s on %s" % (what, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
     if not 1 <= t.shape[-1] <= LN_MAX_C:
         raise BtsAmdError("%s: the normalised axis must have 1..%d elements, got %d" % (what, LN_MAX_C, t.shape[-1]))
     return rs
 
 
-def _ln_vec(t, n, x, what):
-    """An f32 vector of n elements on x's device (or None)."""
-    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != x.device):
-        raise BtsAmdError("%s must be a contiguous f32 tensor of %d elements on %s, got %s %s on %s" % (what, n, x.device, tuple(t.shape), t.dtype, t.device))
-    return t
+def _ln_vec(t, n, dev, what):
+    """Address of an f32 vector of n elements on device dev (None for None)."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise BtsAmdError("%s must be a contiguous f32 tensor of %d elements on device %d, got %s %s on %s" % (what, n, dev, tuple(t.shape), t.dtype, t.device))
+    return t.data_ptr()
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=False):
     """x [..., C] f32 / bf16 (rows evenly strided) -> y = (x - mean) / sqrt(var + eps) * weight + bias, dense, in x's dtype; with
-    want_stats also (mean, rstd), f32 [rows]: what layer_norm_bwd takes."""
+    want_stats (y, stats): stats = f32 [2, rows], the rows' means and reciprocal deviations, which layer_norm_bwd takes."""
+    dev = x.get_device()
+    if dev < 0:
+        _lib.require_gpu(x)
+    if dev != current_device():
+        with torch.cuda.device(dev):
+            return layer_norm_fwd(x, weight, bias, eps, want_stats)
     M, xs = _ln_rows(x, "layer_norm_fwd")
-    Cc = x.shape[-1]
-    _ln_vec(weight, Cc, x, "layer_norm_fwd: weight")
-    _ln_vec(bias, Cc, x, "layer_norm_fwd: bias")
+    Cc, dt = x.shape[-1], dtype_code(x.dtype)
+    w, b = _ln_vec(weight, Cc, dev, "layer_norm_fwd: weight"), _ln_vec(bias, Cc, dev, "layer_norm_fwd: bias")
     if not eps >= 0.0:
         raise BtsAmdError("layer_norm_fwd: eps must be >= 0, got %r" % (eps,))
-    dt = dtype_code(x.dtype)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if want_stats else None
+    stats, mean = None, None
+    if want_stats:
+        stats = torch.empty((2, M), dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
     if M:
         if profiler.ACTIVE is not None:
             profiler.note("layernorm_fwd", "hbm", 2 * M * Cc * x.element_size())
-        with on_device(x):
-            call("bts_layernorm_fwd", _p(x), dt, xs, _p(y), Cc, M, Cc, _p(weight), _p(bias), float(eps), _p(stats[0] if want_stats else None),
-                 _p(stats[1] if want_stats else None), stream_ptr())
-    return (y, stats[0], stats[1]) if want_stats else y
+        call("bts_layernorm_fwd", x.data_ptr(), dt, xs, y.data_ptr(), Cc, M, Cc, w, b, eps, mean, mean + 4 * M if want_stats else None, raw_stream())
+    return (y, stats) if want_stats else y
 
 
-def layer_norm_bwd(dy, x, mean, rstd, weight=None, want_dx=True, want_dweight=True, want_dbias=True):
+def layer_norm_bwd(dy, x, stats, weight=None, want_dx=True, want_dweight=True, want_dbias=True):
     """Gradients (dx, dweight, dbias) of layer_norm_fwd; one that is not wanted is None.  dx is dense, in x's dtype; dweight and dbias are
     f32 [C], sums over all rows in a fixed order."""
+    dev = x.get_device()
+    if dev < 0:
+        _lib.require_gpu(x)
+    if dev != current_device():
+        with torch.cuda.device(dev):
+            return layer_norm_bwd(dy, x, stats, weight, want_dx, want_dweight, want_dbias)
     M, xs = _ln_rows(x, "layer_norm_bwd")
     _, dys = _ln_rows(dy, "layer_norm_bwd: dy", x)
-    Cc = x.shape[-1]
-    _ln_vec(weight, Cc, x, "layer_norm_bwd: weight")
-    for t in (mean, rstd):
-        if t is None:
-            raise BtsAmdError("layer_norm_bwd needs mean and rstd (layer_norm_fwd with want_stats)")
-        _ln_vec(t, M, x, "layer_norm_bwd: mean / rstd")
-    dt = dtype_code(x.dtype)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+    Cc, dt, device = x.shape[-1], dtype_code(x.dtype), x.device
+    if stats is None:
+        raise BtsAmdError("layer_norm_bwd needs the stats of layer_norm_fwd(..., want_stats=True)")
+    mean, w = _ln_vec(stats, 2 * M, dev, "layer_norm_bwd: stats"), _ln_vec(weight, Cc, dev, "layer_norm_bwd: weight")
     make = torch.empty if M else torch.zeros
-    dw = make(Cc, dtype=torch.float32, device=x.device) if want_dweight else None
-    db = make(Cc, dtype=torch.float32, device=x.device) if want_dbias else None
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_dx else None
+    dw = make(Cc, dtype=torch.float32, device=device) if want_dweight else None
+    db = make(Cc, dtype=torch.float32, device=device) if want_dbias else None
     if M and (want_dx or want_dweight or want_dbias):
-        with on_device(x):
-            ws = None
-            if want_dweight or want_dbias:
-                ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc) // 4, dtype=torch.float32, device=x.device)
-            if profiler.ACTIVE is not None:
-                profiler.note("layernorm_bwd", "hbm", M * Cc * x.element_size() * (3 if want_dx else 2))
-            call("bts_layernorm_bwd", _p(dy), dys, _p(x), xs, _p(dx), Cc, dt, M, Cc, _p(weight), _p(mean), _p(rstd), _p(dw), _p(db), _p(ws),
-                 stream_ptr())
+        ws = None
+        if want_dweight or want_dbias:
+            ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc), dtype=torch.uint8, device=device)
+        if profiler.ACTIVE is not None:
+            profiler.note("layernorm_bwd", "hbm", M * Cc * x.element_size() * (3 if want_dx else 2))
+        call("bts_layernorm_bwd", dy.data_ptr(), dys, x.data_ptr(), xs, dx.data_ptr() if want_dx else None, Cc, dt, M, Cc, w, mean, mean + 4 * M,
+             dw.data_ptr() if want_dweight else None, db.data_ptr() if want_dbias else None, ws.data_ptr() if ws is not None else None, raw_stream())
     return dx, dw, db
 
 

@@ -71,8 +71,8 @@ SHAPES = [(1, 1), (3, 2), (5, 3), (1, 7), (33, 8), (257, 16), (70, 17), (100, 33
 @pytest.mark.parametrize("M,C", SHAPES)
 def test_forward_and_backward(M, C, dtype):
     x, w, b, dy = make(M, C, dtype, M * 31 + C)
-    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, stats, w)
     torch.cuda.synchronize()
     r = plain(x, w, b, 1e-5, dy)
     assert y.dtype == dx.dtype == dtype and y.is_contiguous() and dx.is_contiguous() and dw.dtype == db.dtype == torch.float32
@@ -87,8 +87,8 @@ def test_forward_and_backward(M, C, dtype):
 def test_strided_rows_at_any_address(M, C, pad, offset, dtype):
     x, w, b, dy = make(M, C, dtype, 7, pad, offset)
     assert pad == 0 or not x.is_contiguous()
-    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, stats, w)
     r = plain(x, w, b, 1e-5, dy)
     within(y, r["y"], r["tol_y"], "y", HALF[dtype])
     within(dx, r["dx"], r["tol_dx"], "dx", HALF[dtype])
@@ -121,9 +121,9 @@ def test_entry_points_write_only_their_rows():
 @pytest.mark.parametrize("C", [48, 2208])
 def test_only_what_is_asked_for(C, want):
     x, w, b, dy = make(65, C, torch.float32, 11)
-    _, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-    full = ops.layer_norm_bwd(dy, x, mean, rstd, w)
-    part = ops.layer_norm_bwd(dy, x, mean, rstd, w, *want)
+    _, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    full = ops.layer_norm_bwd(dy, x, stats, w)
+    part = ops.layer_norm_bwd(dy, x, stats, w, *want)
     for f, p, k in zip(full, part, want):
         assert (p is None) != k
         assert not k or torch.equal(f, p)
@@ -145,11 +145,11 @@ def test_constant_rows_and_rows_far_from_zero():
     """Variance 0 gives y = bias; a mean of 1000 times the spread loses A / s of the tolerance and no more (no E[x^2] - mean^2)."""
     _, w, b, dy = make(4, 200, torch.float32, 9)
     x = torch.full((4, 200), 3.25, device=DEV)
-    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-    assert torch.equal(y, b.expand(4, 200)) and torch.equal(mean, x[:, 0])
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    assert torch.equal(y, b.expand(4, 200)) and torch.equal(stats[0], x[:, 0])
     x = 1000 + torch.randn(4, 200, device=DEV)
-    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-    dx, _, _ = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    dx, _, _ = ops.layer_norm_bwd(dy, x, stats, w)
     r = plain(x, w, b, 1e-5, dy)
     within(y, r["y"], r["tol_y"], "y")
     within(dx, r["dx"], r["tol_dx"], "dx")
@@ -177,10 +177,10 @@ def test_no_rows():
 
 def test_sums_have_a_fixed_order():
     x, w, b, dy = make(30011, 96, torch.bfloat16, 17)
-    _, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-    first = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    _, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    first = ops.layer_norm_bwd(dy, x, stats, w)
     for _ in range(3):
-        assert all(torch.equal(a, c) for a, c in zip(first, ops.layer_norm_bwd(dy, x, mean, rstd, w)))
+        assert all(torch.equal(a, c) for a, c in zip(first, ops.layer_norm_bwd(dy, x, stats, w)))
 
 
 def test_autograd_against_formula_and_differences():
@@ -265,8 +265,8 @@ def test_captured_pass_replays_on_new_inputs():
     x, dy = x.contiguous(), dy.contiguous()
 
     def step():
-        y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
-        return (y,) + ops.layer_norm_bwd(dy, x, mean, rstd, w)
+        y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+        return (y,) + ops.layer_norm_bwd(dy, x, stats, w)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -311,9 +311,9 @@ def test_refusals_on_the_device():
         layer_norm(x, w, b, -1.0)
     with pytest.raises(BtsAmdError):
         ops.layer_norm_fwd(x.t(), None, None)
-    _, mean, rstd = ops.layer_norm_fwd(x, w, b, want_stats=True)
-    for args in ((dy[:7], x, mean, rstd, w), (dy.bfloat16(), x, mean, rstd, w), (dy, x, None, rstd, w), (dy, x, mean[:7], rstd, w),
-                 (dy, x, mean, rstd.double(), w)):
+    _, stats = ops.layer_norm_fwd(x, w, b, want_stats=True)
+    for args in ((dy[:7], x, stats, w), (dy.bfloat16(), x, stats, w), (dy, x, None, w), (dy, x, stats[:, :7], w), (dy, x, stats.double(), w),
+                 (dy, x, stats, w[:3])):
         with pytest.raises(BtsAmdError):
             ops.layer_norm_bwd(*args)
     # gradients of gradients are refused, not wrong
