@@ -158,12 +158,16 @@ SIGNATURES = {
     "bts_add_to": [_p, _i, _i, _p, _i, _i, _l, _i, _i, _p],
     "bts_adamw_step": [_p, _p, _p, _p, _p, _i, _l, _f, _f, _f, _f, _f, _f, _f, _p, _p],
     "bts_adamw_advance": [_p, _i, _p],
+    "bts_adamw_multi_workspace_bytes": [],
+    "bts_adamw_multi_step": [_p, _p, _l, _p, _i, _p, _p, _p, _p],
+    "bts_adamw_multi_set": [_p, _i, _p, _p],
+    "bts_adamw_multi_moments": [_p, _p, _l, _p, _p, _p, _i, _p],
     "bts_layernorm_fwd": [_p, _i, _l, _p, _l, _l, _i, _p, _p, _f, _p, _p, _p],
     "bts_layernorm_bwd_workspace_bytes": [_i, _l, _i],
     "bts_layernorm_bwd": [_p, _l, _p, _l, _p, _l, _i, _l, _i, _p, _p, _p, _p, _p, _p, _p],
 }
 _LONG_RET = {"bts_silog_workspace_bytes", "bts_bn_stats_workspace_bytes", "bts_eval_workspace_bytes", "bts_bn_bwd_workspace_bytes",
-             "bts_bn_bwd_multi_workspace_bytes", "bts_layernorm_bwd_workspace_bytes"}
+             "bts_bn_bwd_multi_workspace_bytes", "bts_layernorm_bwd_workspace_bytes", "bts_adamw_multi_workspace_bytes"}
 _NO_CHECK = _LONG_RET | {"bts_abi_version", "bts_current_device"}
 
 _lib = None

@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libbts_amd.so")
 SOURCES = ["conv_igemm.hip", "conv_halo.hip", "conv_halo_wide.hip", "conv_wgrad.hip", "conv_wgrad_tr.hip", "conv_c1.hip", "pack.hip", "lpg.hip", "lpg_chain.hip",
-           "elementwise.hip", "layernorm.hip", "evalops.hip"]
+           "elementwise.hip", "layernorm.hip", "adamw.hip", "evalops.hip"]
 HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "conv_common.h"), os.path.join(CSRC, "lpg_math.h"), os.path.join(os.path.dirname(HERE), "include", "bts_amd.h")]
 # packed-fp32-ops off: some forms of the packed f32 instructions that -O3 makes of ordinary float code have given wrong results
 # now and then, with no error; the scalar instructions compute the same values (the host pass warns that it does not know the feature)

@@ -19,29 +19,128 @@ whose per-parameter steps differ inside a group instead of silently rewriting th
 
 Gradients must keep their storage between steps (call ``zero_grad(set_to_none=False)``, the default here):
 the device pointer tables are rebuilt only when a pointer changes.
+
+Three options beyond that, all on `bts_adamw_multi_step` (csrc/adamw.hip; one update launch for ALL groups):
+
+* ``state_bits=8``: the moments of parameters with at least ``min_8bit_size`` elements are held as 8-bit codes, 256 elements (in the
+  parameter's memory order) to a power of two: 2 bytes of state per element instead of 8, read and written once per step.  Codes and
+  scales are ``state[p]['exp_avg_codes' / 'exp_avg_scales' / 'exp_avg_sq_codes' / 'exp_avg_sq_scales']``; ``moments()`` gives the values that
+  they stand for.  Shorter parameters keep 32 bits.  ``state_dict()`` is torch.optim.AdamW's with the f32 values, and loading such a
+  state -- from here, or from the reference's optimizer -- forms the codes again: values that came from codes give the same values.
+* ``max_grad_norm``: the gradients of all groups are scaled by min(1, max_grad_norm / (norm + 1e-6)) inside the step, where norm is their
+  common 2-norm (torch.nn.utils.clip_grad_norm_'s rule; the gradients themselves stay as they are).  No host synchronisation:
+  ``grad_norm`` is a device tensor that every step rewrites.  ``float('inf')`` only measures.
+* bf16 parameters (with bf16 gradients; states stay f32 or 8-bit, the update is formed in f32 and rounded once).
+
+There, states are replaced through ``load_state_dict`` only, and the learning rate is a launch argument: a captured step takes
+``prepared=True`` and ``prepare_step()`` outside the graph, as above.
 """
 import ctypes as C
+import math
+from operator import attrgetter
 
+import numpy as np
 import torch
 
 from . import profiler
-from ._lib import BtsAmdError, call, stream_ptr
+from ._lib import BtsAmdError, call, current_device, raw_stream, require_gpu, stream_ptr
 
 _ROW = 8        # floats per group row (include/bts_amd.h: bts_adamw_advance)
+_WIDE_ROW = 16  # doubles per group row of bts_adamw_multi_step (BTS_ADAMW_ROW)
+_CHUNK, _BLOCK, _MAX_GROUPS = 4096, 256, 64
+_BF16, _8BIT = 1, 2
+_RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("m_scale", "u8"), ("v_scale", "u8"), ("n", "i8"), ("group", "i4"), ("flags", "i4")])
+_RUN_FIRST = "run one step with the same parameters and gradients (zero_grad(set_to_none=False) keeps them)"
+_CODES = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")
+_ptr, _stride, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, attrgetter("grad"), attrgetter("dtype")
+
+
+def _dense(t):
+    """Every element of t's storage span belongs to t once (any order of dimensions)."""
+    expect = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != expect:
+            return False
+        expect *= n
+    return True
+
+
+def _like(flat, off, p):
+    """The p.numel() elements of `flat` from `off` on, with p's shape and p's order in memory."""
+    return torch.as_strided(flat, p.size(), p.stride(), flat.storage_offset() + off)
+
+
+class _Table:
+    """Device tables of one list of tensors: records and chunks of bts_adamw_multi_*, and what they were made from."""
+
+    def __init__(self, records, sizes, device):
+        counts = np.array([-(-n // _CHUNK) for n in sizes], dtype=np.int64)
+        self.n_chunks = int(counts.sum())
+        chunks = np.empty((self.n_chunks, 2), dtype=np.int32)
+        chunks[:, 0] = np.repeat(np.arange(len(sizes), dtype=np.int32), counts)
+        chunks[:, 1] = np.arange(self.n_chunks) - np.repeat(np.cumsum(counts) - counts, counts)
+        self.host = records
+        self.chunks = torch.from_numpy(chunks).to(device)
+        self.stream = None
+        self.upload(device)
+
+    def upload(self, device):
+        """A new device copy of the records: launches in flight may still read the old one."""
+        pinned = torch.empty(self.host.nbytes, dtype=torch.uint8, pin_memory=True)
+        pinned.numpy()[:] = self.host.view(np.uint8)
+        self.records = pinned.to(device, non_blocking=True)
+        self.made_on = raw_stream()
+
+    def use(self):
+        """Called before a launch on the current stream: memory that the allocator gave to another one must outlive this one's work."""
+        if raw_stream() != self.made_on:
+            cur = torch.cuda.current_stream()
+            self.records.record_stream(cur)
+            self.chunks.record_stream(cur)
 
 
 class FusedAdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, min_8bit_size=4096):
+        if state_bits not in (8, 32):
+            raise BtsAmdError("FusedAdamW: state_bits must be 8 or 32, got %r" % (state_bits,))
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise BtsAmdError("FusedAdamW: max_grad_norm must be positive (or None), got %r" % (max_grad_norm,))
+        if int(min_8bit_size) != min_8bit_size or min_8bit_size < 1:
+            raise BtsAmdError("FusedAdamW: min_8bit_size must be a positive whole number, got %r" % (min_8bit_size,))
+        self.state_bits, self.min_8bit_size = state_bits, int(min_8bit_size)
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self._tables = {}
+        self._hyper = None          # [n_groups, 8] f32 on the device (bts_adamw_step), or [n_groups + 1, 16] f64 (bts_adamw_multi_step)
+        self._multi = state_bits == 8 or max_grad_norm is not None
+        self._seen = self._plan = self._state_plan = None
+        self._kept = []             # tables that captured graphs refer to
+        self._scratch = self._norm = None
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
-        self._tables = {}
-        self._hyper = None          # [n_groups, 8] f32 on the device
+
+    def add_param_group(self, param_group):
+        old = getattr(self, "_hyper", None)
+        if old is not None:         # the device rows have one row per group: keep their step counts, make them anew
+            self._refresh_steps()
+            self._hyper = None
+        super().add_param_group(param_group)
+        self._seen = None
+        if not self._multi and any(p.dtype != torch.float32 for p in self.param_groups[-1]["params"]):
+            self._multi, self._tables = True, {}
 
     # ---- device-resident schedule / step counter ------------------------------------------------
     def _device(self):
         for g in self.param_groups:
             for p in g["params"]:
                 return p.device
+        raise BtsAmdError("FusedAdamW has no parameters")
+
+    def _elsewhere(self):
+        """The parameters' device if it is not the current one (launches and streams go by the current device)."""
+        for g in self.param_groups:
+            for p in g["params"]:
+                require_gpu(p)
+                return None if p.device.index == current_device() else p.device
         raise BtsAmdError("FusedAdamW has no parameters")
 
     def _group_step_from_state(self, g):
@@ -59,6 +158,13 @@ class FusedAdamW(torch.optim.Optimizer):
     def _rows(self):
         """The device rows, created on first use from the groups' hyper-parameters and recorded state."""
         if self._hyper is None:
+            if self._multi:
+                rows = np.zeros((len(self.param_groups) + 1, _WIDE_ROW))
+                for r, g in zip(rows, self.param_groups):
+                    r[0], r[3], r[4:6], r[6], r[7] = float(g["lr"]), self._group_step_from_state(g), g["betas"], g["eps"], g["weight_decay"]
+                rows[-1, 0] = math.inf if self.max_grad_norm is None else self.max_grad_norm
+                self._hyper = torch.from_numpy(rows).to(self._device())
+                return self._hyper
             rows = []
             for g in self.param_groups:
                 b1, b2 = g["betas"]
@@ -66,10 +172,25 @@ class FusedAdamW(torch.optim.Optimizer):
             self._hyper = torch.tensor(rows, dtype=torch.float32).to(self._device())
         return self._hyper
 
+    def _host_hyper(self, lrs=None):
+        """The groups' hyper-parameters as bts_adamw_multi_step takes them from the host."""
+        vals = []
+        for gi, g in enumerate(self.param_groups):
+            b1, b2 = g["betas"]
+            vals += [float(g["lr"] if lrs is None else lrs[gi]), float(b1), float(b2), float(g["eps"]), float(g["weight_decay"])]
+        vals.append(math.inf if self.max_grad_norm is None else self.max_grad_norm)
+        return (C.c_double * len(vals))(*vals)
+
     def prepare_step(self, lrs=None):
         """Host side of a step: write the groups' learning rates into the device rows.  Call OUTSIDE a captured
         graph (step() calls it itself unless ``prepared=True``)."""
+        if self._multi and self._elsewhere() is not None:
+            with torch.cuda.device(self._elsewhere()):
+                return self.prepare_step(lrs)
         rows = self._rows()
+        if self._multi:
+            call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), self._host_hyper(lrs), raw_stream())
+            return
         vals = [float(g["lr"] if lrs is None else lrs[gi]) for gi, g in enumerate(self.param_groups)]
         rows[:, 0].copy_(torch.tensor(vals, dtype=torch.float32))
 
@@ -77,7 +198,20 @@ class FusedAdamW(torch.optim.Optimizer):
         """Per-group step counts as python floats (synchronises)."""
         if self._hyper is None:
             return [self._group_step_from_state(g) for g in self.param_groups]
-        return [float(v) for v in self._hyper[:, 3].cpu()]
+        return [float(v) for v in self._hyper[:len(self.param_groups), 3].cpu()]
+
+    def _refresh_steps(self):
+        steps = self.device_steps()
+        for gi, g in enumerate(self.param_groups):
+            for p in g["params"]:
+                st = self.state.get(p)
+                if st:
+                    st["step"] = torch.tensor(steps[gi], dtype=torch.float32)
+
+    @property
+    def grad_norm(self):
+        """The 2-norm of all gradients of the last step (f32, on the device), None without max_grad_norm or before the first step."""
+        return None if self._norm is None else self._norm[0]
 
     # ---- torch.optim.Optimizer surface -------------------------------------------------------------
     def zero_grad(self, set_to_none=False):
@@ -94,21 +228,244 @@ class FusedAdamW(torch.optim.Optimizer):
     def state_dict(self):
         """torch.optim.AdamW layout; the per-parameter ``step`` entries are refreshed from the device counter first
         (they are not touched by step(), which may be running inside a replayed graph)."""
-        steps = self.device_steps()
-        for gi, g in enumerate(self.param_groups):
-            for p in g["params"]:
+        self._refresh_steps()
+        sd = super().state_dict()
+        if self._multi and self.state:
+            ps = [p for g in self.param_groups for p in g["params"]]
+            for i, (p, (m, v)) in enumerate(zip(ps, self.moments())):
                 st = self.state.get(p)
                 if st:
-                    st["step"] = torch.tensor(steps[gi], dtype=torch.float32)
-        return super().state_dict()
+                    sd["state"][i] = {"step": st["step"], "exp_avg": m, "exp_avg_sq": v}
+        return sd
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
         # the moment buffers were replaced and the step count comes from the checkpoint: drop every cached pointer
         # table and rebuild the device rows (step, betas, lr) from what was just loaded
         self._tables = {}
-        self._hyper = None
+        self._hyper = self._seen = self._plan = self._state_plan = None
+        if self._multi:
+            self._load_moments(state_dict)
+        else:
+            for p, st in self.state.items():        # the kernel walks parameter and moments with one index: same order in memory
+                for k in ("exp_avg", "exp_avg_sq"):
+                    if k in st and st[k].stride() != p.stride():
+                        st[k] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(st[k])
         self._rows()
+
+    # ---- 8-bit / multi-tensor form -------------------------------------------------------------------
+    def _load_moments(self, state_dict):
+        ps = [p for g in self.param_groups for p in g["params"]]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        self.state.clear()
+        todo = []
+        for i, p in zip(ids, ps):
+            st = state_dict["state"].get(i)
+            if not st:
+                continue
+            for k in ("exp_avg", "exp_avg_sq"):
+                if k not in st or tuple(st[k].shape) != tuple(p.shape):
+                    raise BtsAmdError("FusedAdamW.load_state_dict: parameter %r needs %s of shape %s" % (i, k, tuple(p.shape)))
+            todo.append((p, st))
+        if not todo:
+            return
+        self._check_parameters([p for p, _ in todo])
+        self._new_state([p for p, _ in todo])
+        for p, st in todo:
+            self.state[p]["step"] = torch.as_tensor(st["step"], dtype=torch.float32).reshape(()).cpu().clone()
+        with torch.cuda.device(self._device()):
+            table, offsets, total = self._state_table()
+            m = torch.empty(total, dtype=torch.float32, device=self._device())
+            v = torch.empty_like(m)
+            at = dict(zip(map(id, self._state_plan[0]), self._state_plan[4]))
+            for p, st in todo:
+                _like(m, at[id(p)], p).copy_(st["exp_avg"])
+                _like(v, at[id(p)], p).copy_(st["exp_avg_sq"])
+            if table.n_chunks:
+                call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, offsets.data_ptr(), m.data_ptr(),
+                     v.data_ptr(), 1, raw_stream())
+
+    def _check_parameters(self, ps):
+        dev = ps[0].device
+        require_gpu(ps[0])
+        if len({id(p) for p in ps}) != len(ps):
+            raise BtsAmdError("FusedAdamW: a parameter appears twice")
+        if len(self.param_groups) > _MAX_GROUPS:
+            raise BtsAmdError("FusedAdamW: at most %d parameter groups" % _MAX_GROUPS)
+        spans = []
+        for p in ps:
+            if p.device != dev or p.dtype not in (torch.float32, torch.bfloat16) or p.layout != torch.strided or not _dense(p):
+                raise BtsAmdError("FusedAdamW needs dense f32 or bf16 parameters on one device, got %s %s %s with strides %s" % (
+                    tuple(p.shape), p.dtype, p.device, p.stride() if p.layout == torch.strided else p.layout))
+            if p.numel():
+                spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise BtsAmdError("FusedAdamW: two parameters overlap in memory")
+
+    def _is_8bit(self, p):
+        return self.state_bits == 8 and p.numel() >= self.min_8bit_size
+
+    def _new_state(self, ps):
+        """Zero states for parameters that have none: one allocation for all codes, one for all scales, one for all f32 moments."""
+        eight, wide = [p for p in ps if self._is_8bit(p)], [p for p in ps if not self._is_8bit(p)]
+        dev = self._device()
+        blocks = [-(-p.numel() // _BLOCK) for p in eight]
+        codes = torch.zeros((2, sum(blocks) * _BLOCK), dtype=torch.uint8, device=dev)
+        scales = torch.full((2, sum(blocks)), 2.0 ** -126, dtype=torch.float32, device=dev)
+        moments = torch.zeros((2, sum(p.numel() for p in wide)), dtype=torch.float32, device=dev)
+        at = 0
+        for p, nb in zip(eight, blocks):
+            n = p.numel()
+            self.state[p] = {"step": torch.zeros((), dtype=torch.float32), "exp_avg_codes": codes[0, at * _BLOCK:at * _BLOCK + n],
+                             "exp_avg_scales": scales[0, at:at + nb], "exp_avg_sq_codes": codes[1, at * _BLOCK:at * _BLOCK + n],
+                             "exp_avg_sq_scales": scales[1, at:at + nb]}
+            at += nb
+        at = 0
+        for p in wide:
+            self.state[p] = {"step": torch.zeros((), dtype=torch.float32), "exp_avg": _like(moments[0], at, p), "exp_avg_sq": _like(moments[1], at, p)}
+            at += p.numel()
+
+    def _state_tensors(self, ps):
+        return [t for p in ps for k, t in self.state[p].items() if k != "step"]
+
+    def _records(self, ps, groups):
+        rec = np.zeros(len(ps), dtype=_RECORD)
+        for i, (p, gi) in enumerate(zip(ps, groups)):
+            st, r = self.state[p], rec[i]
+            flags = _BF16 if p.dtype == torch.bfloat16 else 0
+            if "exp_avg_codes" in st:
+                a, sa, b, sb = (st[k] for k in _CODES)
+                if not (a.dtype == b.dtype == torch.uint8 and sa.dtype == sb.dtype == torch.float32 and a.is_contiguous() and b.is_contiguous()
+                        and a.data_ptr() % 4 == 0 and b.data_ptr() % 4 == 0 and a.numel() == b.numel() == p.numel()
+                        and sa.numel() == sb.numel() == -(-p.numel() // _BLOCK)):
+                    raise BtsAmdError("FusedAdamW: the 8-bit state of a parameter was replaced by something else")
+                r["m"], r["v"], r["m_scale"], r["v_scale"] = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
+                flags |= _8BIT
+            else:
+                a, b = st["exp_avg"], st["exp_avg_sq"]
+                if any(t.dtype != torch.float32 or t.shape != p.shape or t.device != p.device or any(x != y for x, y, n in zip(t.stride(), p.stride(), p.shape) if n != 1) for t in (a, b)):
+                    raise BtsAmdError("FusedAdamW: the state of a parameter was replaced by something that is not f32 in the parameter's layout")
+                r["m"], r["v"] = a.data_ptr(), b.data_ptr()
+            r["p"], r["n"], r["group"], r["flags"] = p.data_ptr(), p.numel(), gi, flags
+        return rec
+
+    def _step_table(self):
+        """The table of all parameters that have a gradient now.  What it was made from is compared every step: addresses and types of
+        parameters and gradients and the gradients' strides; a gradient that moved costs one small upload, anything else a new table."""
+        ps, groups = [], []
+        for gi, g in enumerate(self.param_groups):
+            ps += g["params"]
+            groups += [gi] * len(g["params"])
+        gs = list(map(_grad, ps))
+        if type(None) in set(map(type, gs)):
+            keep = [i for i, g in enumerate(gs) if g is not None]
+            ps, groups, gs = [ps[i] for i in keep], [groups[i] for i in keep], [gs[i] for i in keep]
+        if not ps:
+            return None
+        gptr = list(map(_ptr, gs))
+        seen = (list(map(id, ps)), groups, list(map(_ptr, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
+        if self._plan is not None and seen == self._seen:
+            if gptr == self._gptr:
+                return self._plan
+            self._no_capture("step", _RUN_FIRST)
+            self._plan.host["g"] = gptr
+            self._plan.upload(self._device())
+            self._gptr = gptr
+            return self._plan
+        self._no_capture("step", _RUN_FIRST)
+        self._check_parameters(ps)
+        for p, g in zip(ps, gs):
+            if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or any(a != b for a, b, n in zip(g.stride(), p.stride(), p.shape) if n != 1):
+                raise BtsAmdError("FusedAdamW needs gradients of the parameter's type and layout on its device: parameter %s %s %s, gradient %s %s %s" % (
+                    tuple(p.shape), p.dtype, p.stride(), tuple(g.shape), g.dtype, g.stride() if g.layout == torch.strided else g.layout))
+        fresh = [p for p in ps if not self.state.get(p)]
+        if fresh:
+            self._new_state(fresh)
+            self._state_plan = None
+        rec = self._records(ps, groups)
+        rec["g"] = gptr
+        self._plan = _Table(rec, [p.numel() for p in ps], self._device())
+        self._plan.holds = (ps, self._state_tensors(ps))        # the addresses in the table stay theirs
+        self._seen, self._gptr = seen, gptr
+        self._bytes = sum(p.numel() * (3 * p.element_size() + (4 if self._is_8bit(p) else 16)) for p in ps)
+        return self._plan
+
+    def _no_capture(self, what, how):
+        if torch.cuda.is_current_stream_capturing():
+            raise BtsAmdError("FusedAdamW.%s: device tables cannot be made while a graph is captured -- %s first" % (what, how))
+
+    def _state_table(self):
+        """(table, offsets on the device, elements) of all parameters that have a state, for bts_adamw_multi_moments."""
+        ps = [p for g in self.param_groups for p in g["params"]]
+        offs, at = [], 0
+        for p in ps:
+            offs.append(at)
+            at += p.numel()
+        have = [i for i, p in enumerate(ps) if self.state.get(p)]
+        hp = [ps[i] for i in have]
+        ids = list(map(id, hp))
+        if self._state_plan is None or list(map(id, self._state_plan[0])) != ids:
+            self._no_capture("moments", "call moments() once")
+            table = _Table(self._records(hp, [0] * len(hp)), [p.numel() for p in hp], self._device())
+            offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
+            table.holds = self._state_tensors(hp)
+            self._state_plan = (hp, table, offsets, at, [offs[i] for i in have], len(have) == len(ps))
+        return self._state_plan[1], self._state_plan[2], at
+
+    @torch.no_grad()
+    def moments(self, flat=False):
+        """What the states stand for, in f32: a list of (exp_avg, exp_avg_sq) per parameter in the groups' order, shaped like the parameters --
+        or, with flat, two vectors that hold them one after the other (each in its parameter's memory order).  New memory every time;
+        zeros where a parameter has no state yet.  To be captured into a graph it must have been called once before."""
+        if self._elsewhere() is not None:
+            with torch.cuda.device(self._elsewhere()):
+                return self.moments(flat)
+        table, offsets, total = self._state_table()
+        make = torch.empty if self._state_plan[5] else torch.zeros
+        m = make(total, dtype=torch.float32, device=self._device())
+        v = make(total, dtype=torch.float32, device=self._device())
+        if table.n_chunks:
+            table.use()
+            if torch.cuda.is_current_stream_capturing():
+                self._kept.append(self._state_plan)
+            if profiler.ACTIVE is not None:
+                profiler.note("adamw_moments", "hbm", 10.0 * total)
+            call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, offsets.data_ptr(), m.data_ptr(),
+                 v.data_ptr(), 0, raw_stream())
+        if flat:
+            return m, v
+        out, at = [], 0
+        for g in self.param_groups:
+            for p in g["params"]:
+                out.append((_like(m, at, p), _like(v, at, p)))
+                at += p.numel()
+        return out
+
+    def _step_multi(self, prepared):
+        table = self._step_table()
+        rows = self._rows()
+        hyper = None if prepared else self._host_hyper()
+        norm = None
+        if self.max_grad_norm is not None:
+            if self._norm is None:
+                self._norm = torch.zeros(1, dtype=torch.float32, device=self._device())
+                self._scratch = torch.empty(call("bts_adamw_multi_workspace_bytes") // 8, dtype=torch.float64, device=self._device())
+            norm = self._norm.data_ptr()
+        if table is None or not table.n_chunks:         # no gradient at all: the step count goes on, as bts_adamw_advance does
+            if hyper is not None:
+                call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), hyper, raw_stream())
+            rows[:len(self.param_groups), 3] += 1
+            return
+        table.use()
+        if torch.cuda.is_current_stream_capturing():
+            self._kept.append((table.records, table.chunks, rows))
+        if profiler.ACTIVE is not None:
+            profiler.note("adamw_multi_step", "hbm", float(self._bytes))
+        call("bts_adamw_multi_step", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, rows.data_ptr(), len(self.param_groups), hyper,
+             self._scratch.data_ptr() if norm is not None else None, norm, raw_stream())
+        # parameters were updated through raw pointers: tell autograd / any version-keyed cache
+        torch.autograd.graph.increment_version([p for g in self.param_groups for p in g["params"] if p.grad is not None])
 
     def _table(self, gi, plist):
         st = [self.state[p] for p in plist]
@@ -132,6 +489,11 @@ class FusedAdamW(torch.optim.Optimizer):
     def step(self, closure=None, prepared=False):
         if closure is not None:
             raise BtsAmdError("FusedAdamW.step() does not support a closure (bts_main.py never passes one)")
+        if self._multi:
+            if self._elsewhere() is not None:
+                with torch.cuda.device(self._elsewhere()):
+                    return self._step_multi(prepared)
+            return self._step_multi(prepared)
         if not prepared:
             self.prepare_step()
         rows = self._rows()

@@ -518,6 +518,46 @@ long bts_layernorm_bwd_workspace_bytes(int dtype, long M, int C);
 int bts_layernorm_bwd(const void* dy, long dy_stride, const void* x, long x_stride, void* dx, long dx_stride, int dtype, long M, int C,
                       const float* w, const float* mean, const float* rstd, float* dw, float* db, void* workspace, bts_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * AdamW over many tensors with states in 32 or in 8 bits, f32 or bf16 parameters, optionally clipped by the global gradient norm:
+ *     c = min(1, max_norm / (|g| + 1e-6)) over ALL gradients of the call (1 without clipping), g' = c g
+ *     m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g' g'   (8-bit states: each product and sum rounded to 64 bits, in this order)
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * tensors [n] and chunks [n_chunks][2] = {tensor, i: its elements from BTS_ADAMW_CHUNK i on} are on the DEVICE; every chunk of
+ * every tensor appears once.  8-bit states: m and v are codes, 256 consecutive elements (memory order) share a power of two in
+ * m_scale / v_scale [ceil(n / 256)]; the code arrays are 4-byte aligned and hold whole blocks of 256.  m: e4m3 (largest 448, NaN
+ * 0x7f), v: e5m3 without a sign (code << 7 is a half: largest 61440); the scale is the smallest 2^k, k >= -126, with which the block's
+ * largest magnitude in four significant bits fits.  Rounded to nearest, ties to even, v > 0 never to 0.
+ * rows (device): (n_groups + 1) x BTS_ADAMW_ROW doubles, a group's {lr, 1 - beta1^t, 1 - beta2^t, t, beta1, beta2, eps, weight_decay, and
+ * what a step derives from them}, behind the groups {max_norm, c}.  t lives there, so a replayed hipGraph advances it.
+ * hyper (HOST, or NULL: what rows holds): n_groups x {lr, beta1, beta2, eps, weight_decay}, then max_norm.
+ * workspace (bts_adamw_multi_workspace_bytes) and grad_norm (device, one float): both, or both NULL for no clipping.
+ * ---------------------------------------------------------------------------------- */
+#define BTS_ADAMW_CHUNK 4096
+#define BTS_ADAMW_BLOCK 256
+#define BTS_ADAMW_ROW 16
+#define BTS_ADAMW_MAX_GROUPS 64
+enum { BTS_ADAMW_BF16 = 1 /* parameter and gradient, else f32 */, BTS_ADAMW_8BIT = 2 /* states, else f32 */ };
+typedef struct {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t n;
+    int32_t group, flags;
+} bts_adamw_tensor_t;
+long bts_adamw_multi_workspace_bytes(void);
+int bts_adamw_multi_step(const bts_adamw_tensor_t* tensors, const int32_t* chunks, long n_chunks, double* rows, int n_groups,
+                         const double* hyper, void* workspace, float* grad_norm, bts_stream_t stream);
+/* Writes hyper into rows without a step (the host's half of a step whose kernels replay in a graph). */
+int bts_adamw_multi_set(double* rows, int n_groups, const double* hyper, bts_stream_t stream);
+/* The moments as f32: store = 0 writes what the states stand for to m and v, store = 1 forms the states from m and v (the two undo each
+ * other).  Tensor i begins at offsets[i] (device) elements of m and v.  p and g are not used. */
+int bts_adamw_multi_moments(const bts_adamw_tensor_t* tensors, const int32_t* chunks, long n_chunks, const int64_t* offsets, float* m, float* v,
+                            int store, bts_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

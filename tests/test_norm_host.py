@@ -55,3 +55,61 @@ def test_c_entries_refuse_bad_arguments():
 def test_modules_have_torch_parameters():
     assert [(k, tuple(v.shape)) for k, v in LayerNorm(12).state_dict().items()] == [(k, tuple(v.shape)) for k, v in torch.nn.LayerNorm(12).state_dict().items()]
     assert list(LayerNorm2d(12, bias=False).state_dict()) == ["weight"] and list(LayerNorm2d(12, elementwise_affine=False).state_dict()) == []
+
+
+def test_adamw_options_are_checked():
+    from bts_amd.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(8))
+    for bad in (dict(state_bits=4), dict(state_bits=16), dict(max_grad_norm=0.0), dict(max_grad_norm=-1.0), dict(max_grad_norm=float("nan")),
+                dict(min_8bit_size=0), dict(min_8bit_size=1.5)):
+        with pytest.raises(_lib.BtsAmdError):
+            FusedAdamW([p], **bad)
+    o = FusedAdamW([p], state_bits=8)
+    p.grad = torch.ones(8)
+    with pytest.raises(_lib.BtsAmdError):            # no CPU path
+        o.step()
+
+
+def test_adamw_c_entries_refuse_bad_arguments():
+    lib, p, n = _lib.load(), C.c_void_p(4096), C.c_void_p(0)
+    hyper = (C.c_double * 6)()
+    good = dict(t=p, c=p, nc=1, rows=p, ng=1, h=hyper, ws=p, gn=p, st=n)
+    step = lambda **k: lib.bts_adamw_multi_step(*{**good, **k}.values())   # noqa: E731
+    for bad in (dict(t=n), dict(c=n), dict(nc=0), dict(nc=-1), dict(nc=2 ** 31), dict(rows=n), dict(ng=0), dict(ng=65), dict(ws=n), dict(gn=n),
+                dict(ws=C.c_void_p(4100))):
+        assert step(**bad) == -1, bad
+    assert lib.bts_adamw_multi_set(n, 1, hyper, n) == lib.bts_adamw_multi_set(p, 0, hyper, n) == lib.bts_adamw_multi_set(p, 1, n, n) == -1
+    good_m = dict(t=p, c=p, nc=1, off=p, m=p, v=p, store=0, st=n)
+    moments = lambda **k: lib.bts_adamw_multi_moments(*{**good_m, **k}.values())   # noqa: E731
+    for bad in (dict(t=n), dict(c=n), dict(nc=0), dict(off=n), dict(m=n), dict(v=n), dict(store=2)):
+        assert moments(**bad) == -1, bad
+    assert lib.bts_adamw_multi_workspace_bytes() > 0
+
+
+def test_adamw_record_matches_the_header():
+    from bts_amd import optim
+    src = open(_lib.os.path.join(_lib.os.path.dirname(_lib._HERE), "include", "bts_amd.h")).read()
+    for name, value in (("CHUNK", optim._CHUNK), ("BLOCK", optim._BLOCK), ("ROW", optim._WIDE_ROW), ("MAX_GROUPS", optim._MAX_GROUPS)):
+        assert "#define BTS_ADAMW_%s %d\n" % (name, value) in src
+    assert optim._RECORD.itemsize == 64 and [optim._RECORD.fields[f][1] for f in ("p", "g", "m", "v", "m_scale", "v_scale", "n", "group", "flags")] == [
+        0, 8, 16, 24, 32, 40, 48, 56, 60]
+
+
+def test_the_written_down_8bit_forms():
+    """The tests' own definition: spacing, range and rounding of the two forms."""
+    from tests import adamw_ref as R
+    s, u = R.numbers(True), R.numbers(False)
+    assert s.numel() == 127 and s[-1] == 448 and s[1] == 2.0 ** -9 and u.numel() == 248 and u[-1] == 61440 and u[1] == 2.0 ** -17
+    assert torch.equal(s, torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double())
+    assert torch.equal(u, (torch.arange(248, dtype=torch.int32) << 7).to(torch.int16).view(torch.float16).double())
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(1000, generator=gen, dtype=torch.float64) * 10 ** torch.randn(1000, generator=gen, dtype=torch.float64)
+    for signed in (True, False):
+        a = x if signed else x.abs()
+        y, ks = R.hold(a, signed)
+        for b, k in zip(range(0, 1000, 256), ks):
+            blk, got = a[b:b + 256], y[b:b + 256]
+            assert ((got - blk).abs() <= 2.0 ** -4 * blk.abs() + 2.0 ** (k - (10 if signed else 18))).all()
+            top = 448.0 if signed else 61440.0
+            assert got.abs().max() <= top * 2.0 ** k and got.abs().max() > top * 2.0 ** (k - 1) * 0.96
+        assert torch.equal(R.hold(y, signed)[0], y)
