@@ -20,51 +20,99 @@ namespace {
 
 constexpr int kChunk = 4096;        // elements a block of the update takes: 4 waves x 4 blocks of 256
 constexpr int kBlock = 256;         // elements that share a scale
+constexpr int kAhead = 2;           // blocks that a wave loads before it works on the first
 
+// Addresses come out of the tensor table; told that they are global memory, the compiler takes global instead of flat accesses (which
+// wait for LDS, too).  Four consecutive elements are one access at any element alignment.
+#define GLOBAL_ __attribute__((address_space(1)))
 typedef float f32x4_a4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_a2_t __attribute__((ext_vector_type(2), aligned(2)));
-typedef uint32_t u32_a1_t __attribute__((aligned(1)));
 
-// four consecutive elements from i on (`left` of them exist), f32 or bf16 at an element-aligned address
-__device__ __forceinline__ void load4(const void* base, long i, long left, bool bf16, float* f) {
-    if (left >= 4) {
-        if (bf16) {
-            const u32x2_a2_t u = *(const u32x2_a2_t*)((const uint16_t*)base + i);
-            f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
-            f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+template <bool BF>
+struct Raw4 {
+    u32x4_t u;
+};
+template <>
+struct Raw4<true> {
+    u32x2_t u;
+};
+// elements i .. i + 3 of an f32 / bf16 array; !FULL: only the first `left` of them exist, the others are 0
+template <bool BF, bool FULL>
+__device__ __forceinline__ Raw4<BF> load4(const void* base, long i, long left) {
+    Raw4<BF> r;
+    if constexpr (BF) {
+        const GLOBAL_ uint16_t* p = (const GLOBAL_ uint16_t*)(uintptr_t)base + i;
+        if (FULL || left >= 4) {
+            const u32x2_a2_t t = *(const GLOBAL_ u32x2_a2_t*)p;
+            r.u = (u32x2_t){t.x, t.y};
         } else {
-            const f32x4_a4_t u = *(const f32x4_a4_t*)((const float*)base + i);
-            f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+            r.u = (u32x2_t){0, 0};
+            if (left > 0) r.u.x = p[0];
+            if (left > 1) r.u.x |= (uint32_t)p[1] << 16;
+            if (left > 2) r.u.y = p[2];
         }
     } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = e < left ? (bf16 ? BF16::ld(base, i + e) : F32::ld(base, i + e)) : 0.f;
+        const GLOBAL_ float* p = (const GLOBAL_ float*)(uintptr_t)base + i;
+        if (FULL || left >= 4) {
+            const f32x4_a4_t t = *(const GLOBAL_ f32x4_a4_t*)p;
+            r.u = (u32x4_t){__float_as_uint(t.x), __float_as_uint(t.y), __float_as_uint(t.z), __float_as_uint(t.w)};
+        } else {
+            r.u = (u32x4_t){0, 0, 0, 0};
+            if (left > 0) r.u.x = __float_as_uint(p[0]);
+            if (left > 1) r.u.y = __float_as_uint(p[1]);
+            if (left > 2) r.u.z = __float_as_uint(p[2]);
+        }
+    }
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ void unpack4(const Raw4<BF>& r, float* f) {
+    if constexpr (BF) {
+        f[0] = __uint_as_float(r.u.x << 16); f[1] = __uint_as_float(r.u.x & 0xffff0000u);
+        f[2] = __uint_as_float(r.u.y << 16); f[3] = __uint_as_float(r.u.y & 0xffff0000u);
+    } else {
+        f[0] = __uint_as_float(r.u.x); f[1] = __uint_as_float(r.u.y); f[2] = __uint_as_float(r.u.z); f[3] = __uint_as_float(r.u.w);
     }
 }
-__device__ __forceinline__ void store4(void* base, long i, long left, bool bf16, const float* f) {
-    if (left >= 4) {
-        if (bf16) *(u32x2_a2_t*)((uint16_t*)base + i) = (u32x2_a2_t){pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
-        else *(f32x4_a4_t*)((float*)base + i) = (f32x4_a4_t){f[0], f[1], f[2], f[3]};
+template <bool BF, bool FULL>
+__device__ __forceinline__ void store4(void* base, long i, long left, const float* f) {
+    if constexpr (BF) {
+        GLOBAL_ uint16_t* p = (GLOBAL_ uint16_t*)(uintptr_t)base + i;
+        const uint32_t a = pack_bf16x2(f[0], f[1]), b = pack_bf16x2(f[2], f[3]);
+        if (FULL || left >= 4) *(GLOBAL_ u32x2_a2_t*)p = (u32x2_a2_t){a, b};
+        else {
+            if (left > 0) p[0] = (uint16_t)a;
+            if (left > 1) p[1] = (uint16_t)(a >> 16);
+            if (left > 2) p[2] = (uint16_t)b;
+        }
     } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) { if (bf16) BF16::st(base, i + e, f[e]); else F32::st(base, i + e, f[e]); }
+        GLOBAL_ float* p = (GLOBAL_ float*)(uintptr_t)base + i;
+        if (FULL || left >= 4) *(GLOBAL_ f32x4_a4_t*)p = (f32x4_a4_t){f[0], f[1], f[2], f[3]};
+        else {
+            if (left > 0) p[0] = f[0];
+            if (left > 1) p[1] = f[1];
+            if (left > 2) p[2] = f[2];
+        }
     }
 }
 // four codes; the code arrays are padded to whole blocks of 256, so a word is always there
-__device__ __forceinline__ uint32_t load_codes(const void* base, long i) { return ((const uint32_t*)base)[i >> 2]; }
+__device__ __forceinline__ uint32_t load_codes(const void* base, long i) { return ((const GLOBAL_ uint32_t*)(uintptr_t)base)[i >> 2]; }
+__device__ __forceinline__ void store_codes(void* base, long i, uint32_t c) { ((GLOBAL_ uint32_t*)(uintptr_t)base)[i >> 2] = c; }
+__device__ __forceinline__ float load_scale(const float* base, long b) { return ((const GLOBAL_ float*)(uintptr_t)base)[b]; }
+__device__ __forceinline__ void store_scale(float* base, long b, float v) { ((GLOBAL_ float*)(uintptr_t)base)[b] = v; }
 
 // ---- the 8-bit forms ---------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void decode_m(uint32_t c, float scale, float* f) {
+// the numbers that four codes stand for, without the block's scale
+__device__ __forceinline__ void decode_m(uint32_t c, float* f) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-    f[0] = lo[0] * scale; f[1] = lo[1] * scale; f[2] = hi[0] * scale; f[3] = hi[1] * scale;
+    f[0] = lo[0]; f[1] = lo[1]; f[2] = hi[0]; f[3] = hi[1];
 }
-__device__ __forceinline__ void decode_v(uint32_t c, float scale, float* f) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint16_t h = (uint16_t)(((c >> (8 * e)) & 0xffu) << 7);
-        f[e] = (float)__builtin_bit_cast(_Float16, h) * scale;
-    }
+__device__ __forceinline__ void decode_v(uint32_t c, float* f) {
+    const uint32_t even = (c & 0x00ff00ffu) << 7, odd = ((c >> 8) & 0x00ff00ffu) << 7;      // two halves each
+    f[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)even);
+    f[1] = (float)__builtin_bit_cast(_Float16, (uint16_t)odd);
+    f[2] = (float)__builtin_bit_cast(_Float16, (uint16_t)(even >> 16));
+    f[3] = (float)__builtin_bit_cast(_Float16, (uint16_t)(odd >> 16));
 }
 // |x| rounded to four significant bits, as (biased exponent of a double) << 3 | mantissa: whole numbers in the order of the magnitudes
 __device__ __forceinline__ uint32_t four_bits(double x) {
@@ -88,9 +136,11 @@ __device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
     r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return r[0] > r[1] ? r[0] : r[1];
 }
-// One block of 256 values, four to a lane -> codes and the block's scale.  SIGNED: e4m3, else e5m3.
+// One block of 256 values, four to a lane -> codes (low word) and the block's scale (high word).  SIGNED: e4m3, else e5m3.  Whatever
+// the values are; not inlined, since the update takes it for unusual blocks only.
 template <bool SIGNED>
-__device__ __forceinline__ uint32_t encode(const double* x, float& scale) {
+__device__ __noinline__ uint64_t encode_any(double x0, double x1, double x2, double x3) {
+    const double x[4] = {x0, x1, x2, x3};
     constexpr int kBias = SIGNED ? 7 : 15, kTop = SIGNED ? 8 : 15;       // exponent bias, exponent of the largest number
     uint32_t q[4], top = 0;
 #pragma unroll
@@ -103,7 +153,6 @@ __device__ __forceinline__ uint32_t encode(const double* x, float& scale) {
     // e4m3 ends at 1.75 x 2^8: 1.875 x 2^n takes the next k
     int k = (int)((SIGNED ? top + 1 : top) >> 3) - 1023 - kTop;
     k = k > -126 ? k : -126;
-    scale = __uint_as_float((uint32_t)(k + 127) << 23);
     uint32_t out = 0;
     const int shift = (1023 + k - kBias) << 3;
 #pragma unroll
@@ -117,12 +166,187 @@ __device__ __forceinline__ uint32_t encode(const double* x, float& scale) {
         if (SIGNED) c |= (int)((__builtin_bit_cast(uint64_t, x[e]) >> 56) & 0x80u);
         out |= (uint32_t)c << (8 * e);
     }
-    return out;
+    return out | (uint64_t)(uint32_t)(k + 127) << 55;
+}
+
+// The same for a block whose largest magnitude is neither tiny nor near the end of f32, from the f32 values: rounding to 24 bits
+// first changes the result only where that lands ON a border between two codes, i.e. where the low 19 bits of the f32 value are 0
+// (every border has at most five significant bits).  Those few are moved one step towards the value that they came from.
+__device__ __forceinline__ void off_the_border(const double* x, uint32_t* u) {
+    uint32_t least = u[0] << 13;
+#pragma unroll
+    for (int e = 1; e < 4; ++e) least = least < (u[e] << 13) ? least : (u[e] << 13);
+    if (__any(least == 0)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double d = (double)__uint_as_float(u[e]), ax = __builtin_fabs(x[e]), ad = __builtin_fabs(d);
+            if ((u[e] << 13) == 0) u[e] = ax > ad ? u[e] + 1 : (ax < ad ? u[e] - 1 : u[e]);
+        }
+    }
+}
+constexpr uint32_t kTiny = 27u << 23, kHuge = 0x7f780000u;       // 2^-100; 2^128 in four bits
+__device__ __forceinline__ uint32_t round_four(uint32_t u) { return (u + 0x7ffffu + ((u >> 20) & 1u)) >> 20; }
+
+__device__ __forceinline__ uint32_t encode_m(const double* x, const float* x32, float& scale) {
+    uint32_t u[4], top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(x32[e]);
+    off_the_border(x, u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = top > (u[e] & 0x7fffffffu) ? top : (u[e] & 0x7fffffffu);
+    top = max_dpp(top);
+    if (top < kTiny || top >= kHuge) {
+        const uint64_t r = encode_any<true>(x[0], x[1], x[2], x[3]);
+        scale = __uint_as_float((uint32_t)(r >> 32));
+        return (uint32_t)r;
+    }
+    int k = (int)((round_four(top) + 1) >> 3) - 127 - 8;                   // e4m3 ends at 1.75 x 2^8: 1.875 x 2^n takes the next k
+    k = k > -126 ? k : -126;
+    scale = __uint_as_float((uint32_t)(k + 127) << 23);
+    const float inv = __uint_as_float((uint32_t)(127 - k) << 23);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float(u[0]) * inv, __uint_as_float(u[1]) * inv, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float(u[2]) * inv, __uint_as_float(u[3]) * inv, c, true);
+}
+__device__ __forceinline__ uint32_t encode_v(const double* x, const float* x32, float& scale) {
+    uint32_t u[4], top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(x32[e]);
+    off_the_border(x, u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = top > u[e] ? top : u[e];
+    top = max_dpp(top);
+    if (top < kTiny || top >= kHuge) {
+        const uint64_t r = encode_any<false>(x[0], x[1], x[2], x[3]);
+        scale = __uint_as_float((uint32_t)(r >> 32));
+        return (uint32_t)r;
+    }
+    int k = (int)(round_four(top) >> 3) - 127 - 15;
+    k = k > -126 ? k : -126;
+    scale = __uint_as_float((uint32_t)(k + 127) << 23);
+    const int shift = (127 + k - 15) << 3;
+    int c[4];
+    bool low = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        c[e] = (int)round_four(u[e]) - shift;
+        low |= c[e] < 8;
+    }
+    if (__any(low)) {                                                      // below the normal numbers
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c[e] < 8) {
+                c[e] = (int)multiples(x[e], 17 - k);
+                if (c[e] == 0 && u[e] != 0) c[e] = 1;
+            }
+    }
+    return (uint32_t)(c[0] | (c[1] << 8)) | ((uint32_t)(c[2] | (c[3] << 8)) << 16);
 }
 
 // rows, kRow doubles per group: {lr, 1 - b1^t, 1 - b2^t, t, b1, b2, eps, weight decay} and, formed with the step count, what the update
 // takes: {1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - b1, 1 - b2}; behind the groups {max_norm, c}
 constexpr int kRow = BTS_ADAMW_ROW;
+
+struct Hyper {
+    double b1, b2, a1, a2, clip;
+    float decay, step, rs, eps;
+};
+
+// what one wave reads of one block of 256 elements
+template <bool BF, bool B8>
+struct Block {
+    Raw4<BF> p, g;
+    Raw4<false> m, v;
+    uint32_t mc, vc;
+    float ms, vs;
+};
+template <bool BF, bool B8, bool FULL>
+__device__ __forceinline__ void load_block(const bts_adamw_tensor_t& t, long b0, int lane, Block<BF, B8>& k) {
+    const long i = b0 + lane * 4, left = t.n - i;
+    k.p = load4<BF, FULL>(t.p, i, left);
+    k.g = load4<BF, FULL>(t.g, i, left);
+    if constexpr (B8) {
+        k.mc = load_codes(t.m, i);
+        k.vc = load_codes(t.v, i);
+        k.ms = load_scale(t.m_scale, b0 / kBlock);
+        k.vs = load_scale(t.v_scale, b0 / kBlock);
+    } else {
+        k.m = load4<false, FULL>(t.m, i, left);
+        k.v = load4<false, FULL>(t.v, i, left);
+    }
+}
+template <bool BF, bool B8, bool FULL>
+__device__ __forceinline__ void update_block(const bts_adamw_tensor_t& t, long b0, int lane, const Block<BF, B8>& k, const Hyper& h) {
+    const long i = b0 + lane * 4, left = t.n - i;
+    float p[4], g[4], m32[4], v32[4];
+    unpack4(k.p, p);
+    unpack4(k.g, g);
+    if constexpr (B8) {
+        float mo[4], vo[4], sm, sv;
+        decode_m(k.mc, mo);
+        decode_v(k.vc, vo);
+        const double b1 = h.b1 * (double)k.ms, b2 = h.b2 * (double)k.vs;       // powers of two: (b1 s) x rounds like b1 (s x)
+        double m[4], v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double gd = (double)g[e] * h.clip;
+            m[e] = b1 * (double)mo[e] + h.a1 * gd;               // every product and sum rounded, in this order: with gradients of
+            v[e] = b2 * (double)vo[e] + h.a2 * gd * gd;          // few bits (bf16, zeros) one value in a thousand IS a border
+            if (!FULL && e >= left) m[e] = v[e] = 0.0;
+            m32[e] = (float)m[e];
+            v32[e] = (float)v[e];
+        }
+        store_codes(t.m, i, encode_m(m, m32, sm));
+        store_codes(t.v, i, encode_v(v, v32, sv));
+        if (lane == 0) {
+            store_scale(t.m_scale, b0 / kBlock, sm);
+            store_scale(t.v_scale, b0 / kBlock, sv);
+        }
+    } else {
+        unpack4(k.m, m32);
+        unpack4(k.v, v32);
+        const float b1 = (float)h.b1, b2 = (float)h.b2, a1 = (float)h.a1, a2 = (float)h.a2, c = (float)h.clip;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float gc = g[e] * c;
+            m32[e] = b1 * m32[e] + a1 * gc;
+            v32[e] = b2 * v32[e] + a2 * gc * gc;
+        }
+        store4<false, FULL>(t.m, i, left, m32);
+        store4<false, FULL>(t.v, i, left, v32);
+    }
+    // The hardware's root and reciprocal (each within one step of f32) do where eps keeps the divisor far from the subnormal numbers,
+    // which they flush; otherwise the correctly rounded ones.
+    if (h.eps >= 1e-12f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = fmaf(p[e], h.decay, -h.step * (m32[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v32[e]) * h.rs + h.eps)));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = fmaf(p[e], h.decay, -h.step * (m32[e] / (sqrtf(v32[e]) * h.rs + h.eps)));
+    }
+    store4<BF, FULL>(t.p, i, left, p);                                     // bf16 parameters: the one rounding to fewer bits, to nearest even
+}
+template <bool BF, bool B8>
+__device__ __forceinline__ void update_chunk(const bts_adamw_tensor_t& t, long base, int wave, int lane, const Hyper& h) {
+    if (base + kChunk <= t.n) {
+#pragma unroll 1
+        for (int it = 0; it < 4; it += kAhead) {
+            Block<BF, B8> k[kAhead];                                       // the loads of kAhead blocks before the first use
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) load_block<BF, B8, true>(t, base + ((it + j) * 4 + wave) * kBlock, lane, k[j]);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) update_block<BF, B8, true>(t, base + ((it + j) * 4 + wave) * kBlock, lane, k[j], h);
+        }
+    } else {
+#pragma unroll 1
+        for (int it = 0; it < 4; ++it) {
+            const long b0 = base + (it * 4 + wave) * kBlock;
+            if (b0 >= t.n) break;
+            Block<BF, B8> k;
+            load_block<BF, B8, false>(t, b0, lane, k);
+            update_block<BF, B8, false>(t, b0, lane, k, h);
+        }
+    }
+}
 
 __global__ __launch_bounds__(256) void adamw_multi_kernel(const bts_adamw_tensor_t* __restrict__ tensors, const int2* __restrict__ chunks, long n_chunks,
                                                          const double* __restrict__ rows, int n_groups) {
@@ -130,74 +354,43 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const bts_adamw_tensor
     const int2 ch = chunks[n_chunks - 1 - blockIdx.x];
     const bts_adamw_tensor_t t = tensors[ch.x];
     const double* r = rows + kRow * t.group;
-    const double clip = rows[kRow * n_groups + 1], b1 = r[4], b2 = r[5], a1 = r[11], a2 = r[12];
-    const float decay = (float)r[8], step = (float)r[9], rs = (float)r[10], eps = (float)r[6];
-    const bool bf16 = t.flags & BTS_ADAMW_BF16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Hyper h = {r[4], r[5], r[11], r[12], rows[kRow * n_groups + 1], (float)r[8], (float)r[9], (float)r[10], (float)r[6]};
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long base = (long)ch.y * kChunk;
-#pragma unroll 1
-    for (int it = 0; it < 4; ++it) {
-        const long b0 = base + (it * 4 + wave) * kBlock, i = b0 + lane * 4, left = t.n - i;
-        if (b0 >= t.n) break;
-        float p[4], g[4];
-        load4(t.p, i, left, bf16, p);
-        load4(t.g, i, left, bf16, g);
-        float m32[4], v32[4];
-        if (t.flags & BTS_ADAMW_8BIT) {
-            float mo[4], vo[4], sm, sv;
-            decode_m(load_codes(t.m, i), t.m_scale[b0 / kBlock], mo);
-            decode_v(load_codes(t.v, i), t.v_scale[b0 / kBlock], vo);
-            double m[4], v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double gd = (double)g[e] * clip;
-                m[e] = b1 * (double)mo[e] + a1 * gd;                 // every product and sum rounded, in this order: with gradients of
-                v[e] = b2 * (double)vo[e] + a2 * gd * gd;            // few bits (bf16, zeros) one value in a thousand IS a border
-                if (e >= left) m[e] = v[e] = 0.0;
-                m32[e] = (float)m[e];
-                v32[e] = (float)v[e];
-            }
-            ((uint32_t*)t.m)[i >> 2] = encode<true>(m, sm);
-            ((uint32_t*)t.v)[i >> 2] = encode<false>(v, sv);
-            if (lane == 0) {
-                t.m_scale[b0 / kBlock] = sm;
-                t.v_scale[b0 / kBlock] = sv;
-            }
-        } else {
-            load4(t.m, i, left, false, m32);
-            load4(t.v, i, left, false, v32);
-            const float b1f = (float)b1, b2f = (float)b2, a1f = (float)a1, a2f = (float)a2, c = (float)clip;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float gc = g[e] * c;
-                m32[e] = b1f * m32[e] + a1f * gc;
-                v32[e] = b2f * v32[e] + a2f * gc * gc;
-            }
-            store4(t.m, i, left, false, m32);
-            store4(t.v, i, left, false, v32);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = p[e] * decay - step * (m32[e] / (sqrtf(v32[e]) * rs + eps));
-        store4(t.p, i, left, bf16, p);                                 // bf16 parameters: the one rounding to fewer bits, to nearest even
+    if (t.flags & BTS_ADAMW_8BIT) {
+        if (t.flags & BTS_ADAMW_BF16) update_chunk<true, true>(t, base, wave, lane, h);
+        else update_chunk<false, true>(t, base, wave, lane, h);
+    } else {
+        if (t.flags & BTS_ADAMW_BF16) update_chunk<true, false>(t, base, wave, lane, h);
+        else update_chunk<false, false>(t, base, wave, lane, h);
     }
 }
 
 // sum of squares of every gradient, in f64 (no overflow of g^2, no loss over 10^8 terms): one partial sum per block, fixed order
+template <bool BF>
+__device__ __forceinline__ void add_squares(const bts_adamw_tensor_t& t, long base, double& s) {
+    Raw4<BF> r[4];
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const long i = base + it * 1024 + threadIdx.x * 4, left = t.n - i;
+        r[it] = load4<BF, false>(t.g, i, left);
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        float g[4];
+        unpack4(r[it], g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fma((double)g[e], (double)g[e], s);
+    }
+}
 __global__ __launch_bounds__(256) void adamw_norm_kernel(const bts_adamw_tensor_t* __restrict__ tensors, const int2* __restrict__ chunks, long n_chunks,
                                                         double* __restrict__ partials) {
     double s = 0.0;
     for (long c = blockIdx.x; c < n_chunks; c += gridDim.x) {
         const int2 ch = chunks[c];
         const bts_adamw_tensor_t t = tensors[ch.x];
-#pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            const long i = (long)ch.y * kChunk + it * 1024 + threadIdx.x * 4, left = t.n - i;
-            if (left <= 0) break;
-            float g[4];
-            load4(t.g, i, left, t.flags & BTS_ADAMW_BF16, g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s = fma((double)g[e], (double)g[e], s);
-        }
+        if (t.flags & BTS_ADAMW_BF16) add_squares<true>(t, (long)ch.y * kChunk, s);
+        else add_squares<false>(t, (long)ch.y * kChunk, s);
     }
     __shared__ double red[4];
     s = wave_sum_d(s);
@@ -262,40 +455,44 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const bts_adamw_tens
     const bts_adamw_tensor_t t = tensors[ch.x];
     float* mo = mf + offsets[ch.x];
     float* vo = vf + offsets[ch.x];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 1
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool eight = t.flags & BTS_ADAMW_8BIT;
+#pragma unroll
     for (int it = 0; it < 4; ++it) {
         const long b0 = (long)ch.y * kChunk + (it * 4 + wave) * kBlock, i = b0 + lane * 4, left = t.n - i;
         if (b0 >= t.n) break;
         float m[4], v[4];
         if (store) {
-            load4(mo, i, left, false, m);
-            load4(vo, i, left, false, v);
-            if (t.flags & BTS_ADAMW_8BIT) {
-                double md[4], vd[4];
-                float sm, sv;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { md[e] = m[e]; vd[e] = v[e]; }
-                ((uint32_t*)t.m)[i >> 2] = encode<true>(md, sm);
-                ((uint32_t*)t.v)[i >> 2] = encode<false>(vd, sv);
+            unpack4(load4<false, false>(mo, i, left), m);
+            unpack4(load4<false, false>(vo, i, left), v);
+            if (eight) {
+                const uint64_t rm = encode_any<true>(m[0], m[1], m[2], m[3]), rv = encode_any<false>(v[0], v[1], v[2], v[3]);
+                store_codes(t.m, i, (uint32_t)rm);
+                store_codes(t.v, i, (uint32_t)rv);
                 if (lane == 0) {
-                    t.m_scale[b0 / kBlock] = sm;
-                    t.v_scale[b0 / kBlock] = sv;
+                    store_scale(t.m_scale, b0 / kBlock, __uint_as_float((uint32_t)(rm >> 32)));
+                    store_scale(t.v_scale, b0 / kBlock, __uint_as_float((uint32_t)(rv >> 32)));
                 }
             } else {
-                store4(t.m, i, left, false, m);
-                store4(t.v, i, left, false, v);
+                store4<false, false>(t.m, i, left, m);
+                store4<false, false>(t.v, i, left, v);
             }
         } else {
-            if (t.flags & BTS_ADAMW_8BIT) {
-                decode_m(load_codes(t.m, i), t.m_scale[b0 / kBlock], m);
-                decode_v(load_codes(t.v, i), t.v_scale[b0 / kBlock], v);
+            if (eight) {
+                const float ms = load_scale(t.m_scale, b0 / kBlock), vs = load_scale(t.v_scale, b0 / kBlock);
+                decode_m(load_codes(t.m, i), m);
+                decode_v(load_codes(t.v, i), v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    m[e] *= ms;
+                    v[e] *= vs;
+                }
             } else {
-                load4(t.m, i, left, false, m);
-                load4(t.v, i, left, false, v);
+                unpack4(load4<false, false>(t.m, i, left), m);
+                unpack4(load4<false, false>(t.v, i, left), v);
             }
-            store4(mo, i, left, false, m);
-            store4(vo, i, left, false, v);
+            store4<false, false>(mo, i, left, m);
+            store4<false, false>(vo, i, left, v);
         }
     }
 }

@@ -17,24 +17,38 @@ __all__ = ["layer_norm", "LayerNorm", "LayerNorm2d"]
 
 
 def _rows(t):
-    """t itself where the kernels can walk it (contiguous, evenly strided rows), else a dense copy."""
-    return t if ops.row_stride(t) is not None else t.contiguous()
+    """t itself where the kernels can walk it (contiguous, evenly strided rows), else a dense copy; and what row_stride says of it."""
+    rows = ops.row_stride(t)
+    if rows is None:
+        t = t.contiguous()
+        rows = ops.row_stride(t)
+    return t, rows
+
+
+def _backward(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dy, (_, dys) = _rows(dy)
+    return (*ops.layer_norm_bwd_unchecked(dy, dys, x, ctx.rows, stats, weight, need[0], need[1], need[2]), None)
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x = _rows(x)
-        y, stats = ops.layer_norm_fwd(x, weight, bias, eps, True)
+        x, rows = _rows(x)
+        y, stats = ops.layer_norm_fwd_rows(x, rows, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
+        ctx.rows = rows
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*ops.layer_norm_bwd(_rows(dy), x, stats, weight, need[0], need[1], need[2]), None)
+        # the engine hands over a gradient of y's shape, type and device, on y's device; a graph of this pass is only asked for with
+        # create_graph, and refused where it would be differentiated
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -43,7 +57,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise BtsAmdError("layer_norm: x must have at least one axis")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
-    return ops.layer_norm_fwd(_rows(x), weight, bias, float(eps))
+    return ops.layer_norm_fwd_rows(*_rows(x), weight, bias, float(eps), False)
 
 
 class LayerNorm(nn.LayerNorm):

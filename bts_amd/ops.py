@@ -489,9 +489,7 @@ def _ln_rows(t, what, like=None):
 
 
 def _ln_vec(t, n, dev, what):
-    """Address of an f32 vector of n elements on device dev (None for None)."""
-    if t is None:
-        return None
+    """Address of an f32 vector of n elements on device dev."""
     if t.dtype != torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
         raise BtsAmdError("%s must be a contiguous f32 tensor of %d elements on device %d, got %s %s on %s" % (what, n, dev, tuple(t.shape), t.dtype, t.device))
     return t.data_ptr()
@@ -500,26 +498,33 @@ def _ln_vec(t, n, dev, what):
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=False):
     """x [..., C] f32 / bf16 (rows evenly strided) -> y = (x - mean) / sqrt(var + eps) * weight + bias, dense, in x's dtype; with
     want_stats (y, stats): stats = f32 [2, rows], the rows' means and reciprocal deviations, which layer_norm_bwd takes."""
+    return layer_norm_fwd_rows(x, _ln_rows(x, "layer_norm_fwd"), weight, bias, eps, want_stats)
+
+
+def layer_norm_fwd_rows(x, rows, weight, bias, eps, want_stats):
+    """layer_norm_fwd where row_stride(x) is known."""
     dev = x.get_device()
     if dev < 0:
         _lib.require_gpu(x)
     if dev != current_device():
         with torch.cuda.device(dev):
-            return layer_norm_fwd(x, weight, bias, eps, want_stats)
-    M, xs = _ln_rows(x, "layer_norm_fwd")
+            return layer_norm_fwd_rows(x, rows, weight, bias, eps, want_stats)
+    M, xs = rows
     Cc, dt = x.shape[-1], dtype_code(x.dtype)
-    w, b = _ln_vec(weight, Cc, dev, "layer_norm_fwd: weight"), _ln_vec(bias, Cc, dev, "layer_norm_fwd: bias")
-    if not eps >= 0.0:
-        raise BtsAmdError("layer_norm_fwd: eps must be >= 0, got %r" % (eps,))
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats, mean = None, None
+    w = None if weight is None else _ln_vec(weight, Cc, dev, "layer_norm_fwd: weight")
+    b = None if bias is None else _ln_vec(bias, Cc, dev, "layer_norm_fwd: bias")
+    if not (eps >= 0.0 and 0 < Cc <= LN_MAX_C):
+        raise BtsAmdError("layer_norm_fwd: eps must be >= 0 and the normalised axis have 1..%d elements, got %r and %d" % (LN_MAX_C, eps, Cc))
+    y = torch.empty_like(x) if xs == Cc else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = rstd = mean = None
     if want_stats:
         stats = torch.empty((2, M), dtype=torch.float32, device=x.device)
         mean = stats.data_ptr()
+        rstd = mean + 4 * M
     if M:
         if profiler.ACTIVE is not None:
             profiler.note("layernorm_fwd", "hbm", 2 * M * Cc * x.element_size())
-        call("bts_layernorm_fwd", x.data_ptr(), dt, xs, y.data_ptr(), Cc, M, Cc, w, b, eps, mean, mean + 4 * M if want_stats else None, raw_stream())
+        call("bts_layernorm_fwd", x.data_ptr(), dt, xs, y.data_ptr(), Cc, M, Cc, w, b, eps, mean, rstd, raw_stream())
     return (y, stats) if want_stats else y
 
 
@@ -532,24 +537,43 @@ def layer_norm_bwd(dy, x, stats, weight=None, want_dx=True, want_dweight=True, w
     if dev != current_device():
         with torch.cuda.device(dev):
             return layer_norm_bwd(dy, x, stats, weight, want_dx, want_dweight, want_dbias)
-    M, xs = _ln_rows(x, "layer_norm_bwd")
+    rows = _ln_rows(x, "layer_norm_bwd")
     _, dys = _ln_rows(dy, "layer_norm_bwd: dy", x)
-    Cc, dt, device = x.shape[-1], dtype_code(x.dtype), x.device
     if stats is None:
         raise BtsAmdError("layer_norm_bwd needs the stats of layer_norm_fwd(..., want_stats=True)")
-    mean, w = _ln_vec(stats, 2 * M, dev, "layer_norm_bwd: stats"), _ln_vec(weight, Cc, dev, "layer_norm_bwd: weight")
-    make = torch.empty if M else torch.zeros
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_dx else None
-    dw = make(Cc, dtype=torch.float32, device=device) if want_dweight else None
-    db = make(Cc, dtype=torch.float32, device=device) if want_dbias else None
-    if M and (want_dx or want_dweight or want_dbias):
-        ws = None
-        if want_dweight or want_dbias:
-            ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc), dtype=torch.uint8, device=device)
-        if profiler.ACTIVE is not None:
-            profiler.note("layernorm_bwd", "hbm", M * Cc * x.element_size() * (3 if want_dx else 2))
-        call("bts_layernorm_bwd", dy.data_ptr(), dys, x.data_ptr(), xs, dx.data_ptr() if want_dx else None, Cc, dt, M, Cc, w, mean, mean + 4 * M,
-             dw.data_ptr() if want_dweight else None, db.data_ptr() if want_dbias else None, ws.data_ptr() if ws is not None else None, raw_stream())
+    _ln_vec(stats, 2 * rows[0], dev, "layer_norm_bwd: stats")
+    if weight is not None:
+        _ln_vec(weight, x.shape[-1], dev, "layer_norm_bwd: weight")
+    return layer_norm_bwd_unchecked(dy, dys, x, rows, stats, weight, want_dx, want_dweight, want_dbias)
+
+
+def layer_norm_bwd_unchecked(dy, dys, x, rows, stats, weight, want_dx, want_dweight, want_dbias):
+    """layer_norm_bwd for tensors whose layout is known: `rows`, `dys` = what row_stride says of x, of dy (its stride); x's device is the
+    current one.  The autograd engine runs it on a thread of its own, where every line of Python costs three times what it costs here."""
+    M, xs = rows
+    Cc, dt = x.shape[-1], dtype_code(x.dtype)
+    dx = dw = db = ws = px = pw = pb = pws = None
+    if want_dx:
+        dx = torch.empty_like(x) if xs == Cc else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        px = dx.data_ptr()
+    if want_dweight:
+        dw = torch.empty(Cc, dtype=torch.float32, device=x.device)
+        pw = dw.data_ptr()
+    if want_dbias:
+        db = torch.empty(Cc, dtype=torch.float32, device=x.device)
+        pb = db.data_ptr()
+    if not M:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    if want_dweight or want_dbias:
+        ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc), dtype=torch.uint8, device=x.device)
+        pws = ws.data_ptr()
+    elif not want_dx:
+        return None, None, None
+    if profiler.ACTIVE is not None:
+        profiler.note("layernorm_bwd", "hbm", M * Cc * x.element_size() * (3 if want_dx else 2))
+    mean = stats.data_ptr()
+    call("bts_layernorm_bwd", dy.data_ptr(), dys, x.data_ptr(), xs, px, Cc, dt, M, Cc, None if weight is None else weight.data_ptr(), mean, mean + 4 * M,
+         pw, pb, pws, raw_stream())
     return dx, dw, db
 
 

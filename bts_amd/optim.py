@@ -57,12 +57,18 @@ _ptr, _stride, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, attrg
 
 def _dense(t):
     """Every element of t's storage span belongs to t once (any order of dimensions)."""
+    if t.is_contiguous():
+        return True
     expect = 1
     for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
         if st != expect:
             return False
         expect *= n
     return True
+
+
+def _same_layout(t, p):
+    return t.stride() == p.stride() or all(a == b for a, b, n in zip(t.stride(), p.stride(), p.shape) if n != 1)      # (a size-1 dimension's stride is free)
 
 
 def _like(flat, off, p):
@@ -81,11 +87,11 @@ class _Table:
         chunks[:, 1] = np.arange(self.n_chunks) - np.repeat(np.cumsum(counts) - counts, counts)
         self.host = records
         self.chunks = torch.from_numpy(chunks).to(device)
-        self.stream = None
-        self.upload(device)
+        self.records = torch.from_numpy(records.view(np.uint8)).to(device)
+        self.made_on = raw_stream()
 
     def upload(self, device):
-        """A new device copy of the records: launches in flight may still read the old one."""
+        """A new device copy of the records, without waiting for it: launches in flight may still read the old one."""
         pinned = torch.empty(self.host.nbytes, dtype=torch.uint8, pin_memory=True)
         pinned.numpy()[:] = self.host.view(np.uint8)
         self.records = pinned.to(device, non_blocking=True)
@@ -330,25 +336,24 @@ class FusedAdamW(torch.optim.Optimizer):
         return [t for p in ps for k, t in self.state[p].items() if k != "step"]
 
     def _records(self, ps, groups):
-        rec = np.zeros(len(ps), dtype=_RECORD)
-        for i, (p, gi) in enumerate(zip(ps, groups)):
-            st, r = self.state[p], rec[i]
+        rows = []
+        for p, gi in zip(ps, groups):
+            st, n = self.state[p], p.numel()
             flags = _BF16 if p.dtype == torch.bfloat16 else 0
             if "exp_avg_codes" in st:
                 a, sa, b, sb = (st[k] for k in _CODES)
                 if not (a.dtype == b.dtype == torch.uint8 and sa.dtype == sb.dtype == torch.float32 and a.is_contiguous() and b.is_contiguous()
-                        and a.data_ptr() % 4 == 0 and b.data_ptr() % 4 == 0 and a.numel() == b.numel() == p.numel()
-                        and sa.numel() == sb.numel() == -(-p.numel() // _BLOCK)):
+                        and a.data_ptr() % 4 == 0 and b.data_ptr() % 4 == 0 and a.numel() == b.numel() == n
+                        and sa.numel() == sb.numel() == -(-n // _BLOCK)):
                     raise BtsAmdError("FusedAdamW: the 8-bit state of a parameter was replaced by something else")
-                r["m"], r["v"], r["m_scale"], r["v_scale"] = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
-                flags |= _8BIT
+                rows.append((p.data_ptr(), 0, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), n, gi, flags | _8BIT))
             else:
                 a, b = st["exp_avg"], st["exp_avg_sq"]
-                if any(t.dtype != torch.float32 or t.shape != p.shape or t.device != p.device or any(x != y for x, y, n in zip(t.stride(), p.stride(), p.shape) if n != 1) for t in (a, b)):
-                    raise BtsAmdError("FusedAdamW: the state of a parameter was replaced by something that is not f32 in the parameter's layout")
-                r["m"], r["v"] = a.data_ptr(), b.data_ptr()
-            r["p"], r["n"], r["group"], r["flags"] = p.data_ptr(), p.numel(), gi, flags
-        return rec
+                for t in (a, b):
+                    if t.dtype != torch.float32 or t.shape != p.shape or t.device != p.device or not _same_layout(t, p):
+                        raise BtsAmdError("FusedAdamW: the state of a parameter was replaced by something that is not f32 in the parameter's layout")
+                rows.append((p.data_ptr(), 0, a.data_ptr(), b.data_ptr(), 0, 0, n, gi, flags))
+        return np.array(rows, dtype=_RECORD)
 
     def _step_table(self):
         """The table of all parameters that have a gradient now.  What it was made from is compared every step: addresses and types of
@@ -376,7 +381,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._no_capture("step", _RUN_FIRST)
         self._check_parameters(ps)
         for p, g in zip(ps, gs):
-            if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or any(a != b for a, b, n in zip(g.stride(), p.stride(), p.shape) if n != 1):
+            if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or not _same_layout(g, p):
                 raise BtsAmdError("FusedAdamW needs gradients of the parameter's type and layout on its device: parameter %s %s %s, gradient %s %s %s" % (
                     tuple(p.shape), p.dtype, p.stride(), tuple(g.shape), g.dtype, g.stride() if g.layout == torch.strided else g.layout))
         fresh = [p for p in ps if not self.state.get(p)]
@@ -465,7 +470,7 @@ class FusedAdamW(torch.optim.Optimizer):
         call("bts_adamw_multi_step", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, rows.data_ptr(), len(self.param_groups), hyper,
              self._scratch.data_ptr() if norm is not None else None, norm, raw_stream())
         # parameters were updated through raw pointers: tell autograd / any version-keyed cache
-        torch.autograd.graph.increment_version([p for g in self.param_groups for p in g["params"] if p.grad is not None])
+        torch.autograd.graph.increment_version(table.holds[0])
 
     def _table(self, gi, plist):
         st = [self.state[p] for p in plist]
