@@ -505,7 +505,7 @@ extern "C" long bts_adamw_multi_workspace_bytes(void) { return kNormBlocks * (lo
 
 extern "C" int bts_adamw_multi_step(const bts_adamw_tensor_t* tensors, const int32_t* chunks, long n_chunks, double* rows, int n_groups,
                                     const double* hyper, void* workspace, float* grad_norm, bts_stream_t stream) {
-    BTS_CHECK_ARG(tensors && chunks && rows && n_chunks > 0 && n_chunks <= 0x7fffffff && n_groups > 0 && n_groups <= BTS_ADAMW_MAX_GROUPS);
+    BTS_CHECK_ARG(tensors && chunks && rows && n_chunks > 0 && n_chunks <= 0xffffff && n_groups > 0 && n_groups <= BTS_ADAMW_MAX_GROUPS);
     BTS_CHECK_ARG(!workspace == !grad_norm && ((uintptr_t)workspace & 7) == 0);
     hipStream_t st = (hipStream_t)stream;
     HostHyper hh = {};
@@ -540,7 +540,7 @@ extern "C" int bts_adamw_multi_set(double* rows, int n_groups, const double* hyp
 
 extern "C" int bts_adamw_multi_moments(const bts_adamw_tensor_t* tensors, const int32_t* chunks, long n_chunks, const int64_t* offsets, float* m, float* v,
                                        int store, bts_stream_t stream) {
-    BTS_CHECK_ARG(tensors && chunks && offsets && m && v && n_chunks > 0 && n_chunks <= 0x7fffffff && (store == 0 || store == 1));
+    BTS_CHECK_ARG(tensors && chunks && offsets && m && v && n_chunks > 0 && n_chunks <= 0xffffff && (store == 0 || store == 1));
     hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)n_chunks), dim3(256), 0, (hipStream_t)stream, tensors, (const int2*)chunks,
                        (const long*)offsets, m, v, store);
     BTS_LAUNCH_CHECK();

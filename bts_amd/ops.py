@@ -465,6 +465,8 @@ def row_stride(t):
         return t.numel() // Cc if Cc else 0, Cc
     if Cc > 1 and t.stride(-1) != 1:
         return None
+    if t.dim() == 2 and t.shape[0] > 1:
+        return t.shape[0], t.stride(0)
     rows, stride = 1, None
     for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if n == 1:

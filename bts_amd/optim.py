@@ -67,6 +67,11 @@ def _dense(t):
     return True
 
 
+def _room(t):
+    """Bytes of t's storage from t's first element on."""
+    return t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+
+
 def _same_layout(t, p):
     return t.stride() == p.stride() or all(a == b for a, b, n in zip(t.stride(), p.stride(), p.shape) if n != 1)      # (a size-1 dimension's stride is free)
 
@@ -113,16 +118,32 @@ class FusedAdamW(torch.optim.Optimizer):
             raise BtsAmdError("FusedAdamW: max_grad_norm must be positive (or None), got %r" % (max_grad_norm,))
         if int(min_8bit_size) != min_8bit_size or min_8bit_size < 1:
             raise BtsAmdError("FusedAdamW: min_8bit_size must be a positive whole number, got %r" % (min_8bit_size,))
-        self.state_bits, self.min_8bit_size = state_bits, int(min_8bit_size)
-        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self._options = (state_bits, int(min_8bit_size), None if max_grad_norm is None else float(max_grad_norm))
+        self._multi = state_bits == 8 or max_grad_norm is not None
+        self._forget()
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+        super().__init__(params, defaults)
+
+    # the options are the constructor's: the layout of states and device rows goes by them
+    state_bits = property(lambda self: self._options[0])
+    min_8bit_size = property(lambda self: self._options[1])
+    max_grad_norm = property(lambda self: self._options[2])
+
+    def _forget(self):
         self._tables = {}
         self._hyper = None          # [n_groups, 8] f32 on the device (bts_adamw_step), or [n_groups + 1, 16] f64 (bts_adamw_multi_step)
-        self._multi = state_bits == 8 or max_grad_norm is not None
         self._seen = self._plan = self._state_plan = None
         self._kept = []             # tables that captured graphs refer to
         self._scratch = self._norm = None
-        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
-        super().__init__(params, defaults)
+
+    def __getstate__(self):         # copies and pickles: states with their step counts, nothing that holds addresses
+        self._refresh_steps()
+        return {**super().__getstate__(), "_options": self._options, "_multi": self._multi}
+
+    def __setstate__(self, state):  # (load_state_dict calls it too, with the loaded states and groups)
+        super().__setstate__(state)
+        if "_options" in state:
+            self._forget()
 
     def add_param_group(self, param_group):
         old = getattr(self, "_hyper", None)
@@ -344,7 +365,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 a, sa, b, sb = (st[k] for k in _CODES)
                 if not (a.dtype == b.dtype == torch.uint8 and sa.dtype == sb.dtype == torch.float32 and a.is_contiguous() and b.is_contiguous()
                         and a.data_ptr() % 4 == 0 and b.data_ptr() % 4 == 0 and a.numel() == b.numel() == n
-                        and sa.numel() == sb.numel() == -(-n // _BLOCK)):
+                        and sa.numel() == sb.numel() == -(-n // _BLOCK) and _room(a) >= sa.numel() * _BLOCK and _room(b) >= sa.numel() * _BLOCK):
                     raise BtsAmdError("FusedAdamW: the 8-bit state of a parameter was replaced by something else")
                 rows.append((p.data_ptr(), 0, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), n, gi, flags | _8BIT))
             else:

@@ -524,7 +524,7 @@ int bts_layernorm_bwd(const void* dy, long dy_stride, const void* x, long x_stri
  *     m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g' g'   (8-bit states: each product and sum rounded to 64 bits, in this order)
  *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * tensors [n] and chunks [n_chunks][2] = {tensor, i: its elements from BTS_ADAMW_CHUNK i on} are on the DEVICE; every chunk of
- * every tensor appears once.  8-bit states: m and v are codes, 256 consecutive elements (memory order) share a power of two in
+ * every tensor appears once (n_chunks < 2^24: a grid holds 2^32 threads).  8-bit states: m and v are codes, 256 consecutive elements (memory order) share a power of two in
  * m_scale / v_scale [ceil(n / 256)]; the code arrays are 4-byte aligned and hold whole blocks of 256.  m: e4m3 (largest 448, NaN
  * 0x7f), v: e5m3 without a sign (code << 7 is a half: largest 61440); the scale is the smallest 2^k, k >= -126, with which the block's
  * largest magnitude in four significant bits fits.  Rounded to nearest, ties to even, v > 0 never to 0.

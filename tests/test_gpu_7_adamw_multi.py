@@ -428,6 +428,24 @@ def test_groups_added_later():
     assert opt.device_steps() == [3.0, 2.0, 1.0]
 
 
+@pytest.mark.parametrize("kw", [dict(state_bits=8, min_8bit_size=1), dict(state_bits=8, max_grad_norm=1.0), dict()])
+def test_copies_go_on_by_themselves(kw):
+    """copy.deepcopy of a model with its optimizer: the copy has the states and the step count, and memory of its own."""
+    ps = tensors([5001, 40], torch.float32, 31)
+    opt = optimizer(ps, 1, **kw)
+    feed(ps, 1)
+    opt.step()
+    qs, twin = copy.deepcopy((ps, opt))
+    assert twin.device_steps() == [1.0, 1.0] and twin.param_groups[0]["params"][0] is qs[0]
+    was = [p.detach().clone() for p in ps]
+    feed(qs, 2)
+    twin.step()
+    assert all(torch.equal(p, w) for p, w in zip(ps, was))
+    feed(ps, 2)
+    opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and not torch.equal(ps[0], was[0])
+
+
 def test_offsets_beyond_32_bits():
     """A bf16 parameter of 2^31 + 4613 elements: its last blocks are updated like those of a short tensor."""
     n, tail = 2 ** 31 + 4613, 5000

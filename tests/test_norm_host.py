@@ -65,6 +65,8 @@ def test_adamw_options_are_checked():
         with pytest.raises(_lib.BtsAmdError):
             FusedAdamW([p], **bad)
     o = FusedAdamW([p], state_bits=8)
+    with pytest.raises(AttributeError):              # options are fixed: states and rows are laid out by them
+        o.max_grad_norm = 1.0
     p.grad = torch.ones(8)
     with pytest.raises(_lib.BtsAmdError):            # no CPU path
         o.step()
@@ -75,7 +77,7 @@ def test_adamw_c_entries_refuse_bad_arguments():
     hyper = (C.c_double * 6)()
     good = dict(t=p, c=p, nc=1, rows=p, ng=1, h=hyper, ws=p, gn=p, st=n)
     step = lambda **k: lib.bts_adamw_multi_step(*{**good, **k}.values())   # noqa: E731
-    for bad in (dict(t=n), dict(c=n), dict(nc=0), dict(nc=-1), dict(nc=2 ** 31), dict(rows=n), dict(ng=0), dict(ng=65), dict(ws=n), dict(gn=n),
+    for bad in (dict(t=n), dict(c=n), dict(nc=0), dict(nc=-1), dict(nc=2 ** 24), dict(rows=n), dict(ng=0), dict(ng=65), dict(ws=n), dict(gn=n),
                 dict(ws=C.c_void_p(4100))):
         assert step(**bad) == -1, bad
     assert lib.bts_adamw_multi_set(n, 1, hyper, n) == lib.bts_adamw_multi_set(p, 0, hyper, n) == lib.bts_adamw_multi_set(p, 1, n, n) == -1
