@@ -115,7 +115,8 @@ def parse():
     ap.add_argument("--graph", type=int, default=1, help="capture the train step in a hipGraph (N=1 only; falls back to eager)")
     ap.add_argument("--cudnn-benchmark", type=int, default=1, help="torch.backends.cudnn.benchmark: ATen asks MIOpen's find API (which, in "
                     "find mode `fast`, answers from the recorded results) instead of its immediate-mode heuristic")
-    ap.add_argument("--optimizer", default="bts", choices=["bts", "torch"], help="bts = fused HIP AdamW (bts_adamw_step)")
+    ap.add_argument("--optimizer", default="bts", choices=["bts", "bts8", "torch"], help="bts = fused HIP AdamW (bts_adamw_step); bts8 = with "
+                    "8-bit states (bts_adamw_multi_step)")
     ap.add_argument("--mode", default="train", choices=["train", "infer"],
                     help="infer = BASELINE.json configs[4]: no-grad forward, DenseNet161 704x1216 batch 32 (secondary config)")
     ap.add_argument("--backend", default="nccl", help="torch.distributed backend (nccl = RCCL); gloo only for plumbing tests")
@@ -786,10 +787,10 @@ def main():
     lr_t = torch.tensor(1e-4, device=dev)      # capturable optimizers read lr from a device tensor
     groups = [{"params": [p for p in model.encoder.parameters() if p.requires_grad], "weight_decay": 1e-2},
               {"params": list(model.decoder.parameters()), "weight_decay": 0.0}]       # bts_main.py:371-373
-    own_opt = args.optimizer == "bts"
+    own_opt = args.optimizer in ("bts", "bts8")
     if own_opt:
         from bts_amd.optim import FusedAdamW
-        opt = FusedAdamW(groups, lr=1e-4, eps=1e-3)
+        opt = FusedAdamW(groups, lr=1e-4, eps=1e-3, state_bits=8 if args.optimizer == "bts8" else 32)
     else:
         opt = torch.optim.AdamW(groups, lr=lr_t if use_graph else 1e-4, eps=1e-3, fused=True, capturable=use_graph)
     crit = silog_loss(0.85)
@@ -1002,7 +1003,7 @@ def main():
                        "global_batch": args.batch * world, "parallelism": "dp%d" % world, "grad_exchange": ("none" if not multi else ("torch DDP over %s" % args.backend if reducer is None else "bts GradAllReducer over %s" % args.backend)),
                        "encoder": "stock PyTorch-ROCm (%s autocast, %s, PYTORCH_MIOPEN_SUGGEST_NHWC=%s (BatchNorm: %s), cudnn.benchmark=%d, MIOPEN_FIND_MODE=%s, %s)" % (
                            args.dtype, "channels_last" if args.channels_last else "contiguous NCHW", os.environ.get("PYTORCH_MIOPEN_SUGGEST_NHWC", "unset"), os.environ.get("PYTORCH_MIOPEN_SUGGEST_NHWC_BATCHNORM", "unset"),
-                           args.cudnn_benchmark, os.environ.get("MIOPEN_FIND_MODE", "unset"), miopen_db_note(args)), "decoder": "HIP kernels via libbts_amd.so", "launch": graph_note, "optimizer": "bts_adamw_step (fused HIP)" if own_opt else "torch.optim.AdamW(fused)",
+                           args.cudnn_benchmark, os.environ.get("MIOPEN_FIND_MODE", "unset"), miopen_db_note(args)), "decoder": "HIP kernels via libbts_amd.so", "launch": graph_note, "optimizer": {"bts": "bts_adamw_step (fused HIP)", "bts8": "bts_adamw_multi_step (fused HIP, 8-bit states)"}.get(args.optimizer, "torch.optim.AdamW(fused)"),
                        "final_loss": round(final_loss, 5)},
         }
         if roof is not None:

@@ -36,6 +36,7 @@ There, states are replaced through ``load_state_dict`` only, and the learning ra
 ``prepared=True`` and ``prepare_step()`` outside the graph, as above.
 """
 import ctypes as C
+import itertools
 import math
 from operator import attrgetter
 
@@ -91,6 +92,7 @@ class _Table:
         chunks[:, 0] = np.repeat(np.arange(len(sizes), dtype=np.int32), counts)
         chunks[:, 1] = np.arange(self.n_chunks) - np.repeat(np.cumsum(counts) - counts, counts)
         self.host = records
+        self.holds = self.offsets = None        # what must live as long as the addresses; begin of each tensor in flat moments
         self.chunks = torch.from_numpy(chunks).to(device)
         self.records = torch.from_numpy(records.view(np.uint8)).to(device)
         self.made_on = raw_stream()
@@ -106,8 +108,9 @@ class _Table:
         """Called before a launch on the current stream: memory that the allocator gave to another one must outlive this one's work."""
         if raw_stream() != self.made_on:
             cur = torch.cuda.current_stream()
-            self.records.record_stream(cur)
-            self.chunks.record_stream(cur)
+            for t in (self.records, self.chunks, self.offsets):
+                if t is not None:
+                    t.record_stream(cur)
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -301,16 +304,16 @@ class FusedAdamW(torch.optim.Optimizer):
         for p, st in todo:
             self.state[p]["step"] = torch.as_tensor(st["step"], dtype=torch.float32).reshape(()).cpu().clone()
         with torch.cuda.device(self._device()):
-            table, offsets, total = self._state_table()
-            m = torch.empty(total, dtype=torch.float32, device=self._device())
+            plan = self._state_table()
+            table = plan["table"]
+            m = torch.empty(plan["total"], dtype=torch.float32, device=self._device())
             v = torch.empty_like(m)
-            at = dict(zip(map(id, self._state_plan[0]), self._state_plan[4]))
             for p, st in todo:
-                _like(m, at[id(p)], p).copy_(st["exp_avg"])
-                _like(v, at[id(p)], p).copy_(st["exp_avg_sq"])
+                _like(m, plan["at"][id(p)], p).copy_(st["exp_avg"])
+                _like(v, plan["at"][id(p)], p).copy_(st["exp_avg_sq"])
             if table.n_chunks:
-                call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, offsets.data_ptr(), m.data_ptr(),
-                     v.data_ptr(), 1, raw_stream())
+                call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
+                     m.data_ptr(), v.data_ptr(), 1, raw_stream())
 
     def _check_parameters(self, ps):
         dev = ps[0].device
@@ -422,22 +425,20 @@ class FusedAdamW(torch.optim.Optimizer):
             raise BtsAmdError("FusedAdamW.%s: device tables cannot be made while a graph is captured -- %s first" % (what, how))
 
     def _state_table(self):
-        """(table, offsets on the device, elements) of all parameters that have a state, for bts_adamw_multi_moments."""
+        """The table of all parameters that have a state, for bts_adamw_multi_moments, and where each begins in flat moments."""
         ps = [p for g in self.param_groups for p in g["params"]]
-        offs, at = [], 0
-        for p in ps:
-            offs.append(at)
-            at += p.numel()
-        have = [i for i, p in enumerate(ps) if self.state.get(p)]
-        hp = [ps[i] for i in have]
-        ids = list(map(id, hp))
-        if self._state_plan is None or list(map(id, self._state_plan[0])) != ids:
+        key = (list(map(id, ps)), len(self.state))
+        if self._state_plan is None or self._state_plan["key"] != key:
             self._no_capture("moments", "call moments() once")
-            table = _Table(self._records(hp, [0] * len(hp)), [p.numel() for p in hp], self._device())
-            offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
-            table.holds = self._state_tensors(hp)
-            self._state_plan = (hp, table, offsets, at, [offs[i] for i in have], len(have) == len(ps))
-        return self._state_plan[1], self._state_plan[2], at
+            sizes = [p.numel() for p in ps]
+            offs = [0] + list(itertools.accumulate(sizes))
+            have = [i for i, p in enumerate(ps) if self.state.get(p)]
+            hp = [ps[i] for i in have]
+            table = _Table(self._records(hp, [0] * len(hp)), [sizes[i] for i in have], self._device())
+            table.holds = (ps, self._state_tensors(hp))
+            table.offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
+            self._state_plan = {"key": key, "table": table, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "all": len(have) == len(ps)}
+        return self._state_plan
 
     @torch.no_grad()
     def moments(self, flat=False):
@@ -447,26 +448,20 @@ class FusedAdamW(torch.optim.Optimizer):
         if self._elsewhere() is not None:
             with torch.cuda.device(self._elsewhere()):
                 return self.moments(flat)
-        table, offsets, total = self._state_table()
-        make = torch.empty if self._state_plan[5] else torch.zeros
-        m = make(total, dtype=torch.float32, device=self._device())
-        v = make(total, dtype=torch.float32, device=self._device())
+        plan = self._state_table()
+        table, total = plan["table"], plan["total"]
+        m, v = ((torch.empty if plan["all"] else torch.zeros)(total, dtype=torch.float32, device=self._device()) for _ in range(2))
         if table.n_chunks:
             table.use()
             if torch.cuda.is_current_stream_capturing():
-                self._kept.append(self._state_plan)
+                self._kept.append((table.records, table.chunks, table.offsets))
             if profiler.ACTIVE is not None:
                 profiler.note("adamw_moments", "hbm", 10.0 * total)
-            call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, offsets.data_ptr(), m.data_ptr(),
-                 v.data_ptr(), 0, raw_stream())
+            call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
+                 m.data_ptr(), v.data_ptr(), 0, raw_stream())
         if flat:
             return m, v
-        out, at = [], 0
-        for g in self.param_groups:
-            for p in g["params"]:
-                out.append((_like(m, at, p), _like(v, at, p)))
-                at += p.numel()
-        return out
+        return [(_like(m, plan["at"][id(p)], p), _like(v, plan["at"][id(p)], p)) for g in self.param_groups for p in g["params"]]
 
     def _step_multi(self, prepared):
         table = self._step_table()
