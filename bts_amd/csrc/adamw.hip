@@ -20,7 +20,9 @@ namespace {
 
 constexpr int kChunk = 4096;        // elements a block of the update takes: 4 waves x 4 blocks of 256
 constexpr int kBlock = 256;         // elements that share a scale
-constexpr int kAhead = 2;           // blocks that a wave loads before it works on the first
+// Blocks that a wave loads before it works on the first.  112.8 M f32 / 16.3 M bf16 parameters with 8-bit states, us: 1 (54 registers)
+// 334 / 36.4, 2 (68) 332 / 35.0, 4 (106) 328 / 37.2.
+constexpr int kAhead = 2;
 
 // Addresses come out of the tensor table; told that they are global memory, the compiler takes global instead of flat accesses (which
 // wait for LDS, too).  Four consecutive elements are one access at any element alignment.
@@ -348,6 +350,10 @@ __device__ __forceinline__ void update_chunk(const bts_adamw_tensor_t& t, long b
     }
 }
 
+// One block per chunk: the tensors' sizes differ by five orders of magnitude, equal chunks make equal blocks.  Bound by memory: 550 tensors,
+// 47.0 M f32 parameters with 8-bit states take 157-168 us for 752 MB (4.5-4.8 TB/s; a large copy reaches 4.7-5.1) at 51 VALU instructions an
+// element, 61 us of issue; counted traffic is 484 MB read, 288 MB written.  16.3 M bf16: 35 us, 163 MB.  20.5 M bf16 parameters with
+// 32-bit states: 90 us, 451 MB.  (With flat accesses, one path for all types and the general encoder: 194, 71 and 98 us.)
 __global__ __launch_bounds__(256) void adamw_multi_kernel(const bts_adamw_tensor_t* __restrict__ tensors, const int2* __restrict__ chunks, long n_chunks,
                                                          const double* __restrict__ rows, int n_groups) {
     // last chunk first: behind a norm pass the gradients that were read last are the ones that the cache still holds
@@ -366,7 +372,8 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const bts_adamw_tensor
     }
 }
 
-// sum of squares of every gradient, in f64 (no overflow of g^2, no loss over 10^8 terms): one partial sum per block, fixed order
+// sum of squares of every gradient, in f64 (no overflow of g^2, no loss over 10^8 terms): one partial sum per block, fixed order.
+// 112.8 M f32 gradients: 54 us.
 template <bool BF>
 __device__ __forceinline__ void add_squares(const bts_adamw_tensor_t& t, long base, double& s) {
     Raw4<BF> r[4];
@@ -448,6 +455,7 @@ __global__ __launch_bounds__(1024) void adamw_begin_kernel(double* __restrict__ 
     }
 }
 
+// 47.0 M elements: 95 us for 470 MB.
 // the moments as f32 values (store = 0: states -> m, v; 1: m, v -> states); offsets[t]: where tensor t begins in m and v
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const bts_adamw_tensor_t* __restrict__ tensors, const int2* __restrict__ chunks,
                                                            const long* __restrict__ offsets, float* __restrict__ mf, float* __restrict__ vf, int store) {

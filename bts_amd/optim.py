@@ -308,9 +308,7 @@ class FusedAdamW(torch.optim.Optimizer):
             table = plan["table"]
             m = torch.empty(plan["total"], dtype=torch.float32, device=self._device())
             v = torch.empty_like(m)
-            for p, st in todo:
-                _like(m, plan["at"][id(p)], p).copy_(st["exp_avg"])
-                _like(v, plan["at"][id(p)], p).copy_(st["exp_avg_sq"])
+            torch._foreach_copy_([_like(t, plan["at"][id(p)], p) for t in (m, v) for p, _ in todo], [st[k] for k in ("exp_avg", "exp_avg_sq") for _, st in todo])
             if table.n_chunks:
                 call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
                      m.data_ptr(), v.data_ptr(), 1, raw_stream())

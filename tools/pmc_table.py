@@ -24,7 +24,7 @@ def rows(path, counter):
     return out
 
 
-OURS = re.compile(r"^(conv_|lpg|bn_|affine|act_bwd|add_to|nchw|nhwc|silog|adamw)")
+OURS = re.compile(r"^(conv_|lpg|bn_|affine|act_bwd|add_to|nchw|nhwc|silog|adamw|ln_)")
 
 
 def main():
