@@ -33,7 +33,8 @@ Three options beyond that, all on `bts_adamw_multi_step` (csrc/adamw.hip; one up
 * bf16 parameters (with bf16 gradients; states stay f32 or 8-bit, the update is formed in f32 and rounded once).
 
 There, states are replaced through ``load_state_dict`` only, and the learning rate is a launch argument: a captured step takes
-``prepared=True`` and ``prepare_step()`` outside the graph, as above.
+``prepared=True`` and ``prepare_step()`` outside the graph, as above.  A captured step works on the gradients, states and step counts that it was
+captured with: capture again after ``load_state_dict`` or ``add_param_group``.
 """
 import ctypes as C
 import itertools
@@ -136,7 +137,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._tables = {}
         self._hyper = None          # [n_groups, 8] f32 on the device (bts_adamw_step), or [n_groups + 1, 16] f64 (bts_adamw_multi_step)
         self._seen = self._plan = self._state_plan = None
-        self._kept = []             # tables that captured graphs refer to
+        self._kept = []             # what captured graphs refer to
         self._scratch = self._norm = None
 
     def __getstate__(self):         # copies and pickles: states with their step counts, nothing that holds addresses
@@ -452,7 +453,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if table.n_chunks:
             table.use()
             if torch.cuda.is_current_stream_capturing():
-                self._kept.append((table.records, table.chunks, table.offsets))
+                self._kept.append((table.records, table.chunks, table.offsets, table.holds))
             if profiler.ACTIVE is not None:
                 profiler.note("adamw_moments", "hbm", 10.0 * total)
             call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
@@ -475,10 +476,12 @@ class FusedAdamW(torch.optim.Optimizer):
             if hyper is not None:
                 call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), hyper, raw_stream())
             rows[:len(self.param_groups), 3] += 1
+            if norm is not None:
+                self._norm.zero_()
             return
         table.use()
         if torch.cuda.is_current_stream_capturing():
-            self._kept.append((table.records, table.chunks, rows))
+            self._kept.append((table.records, table.chunks, rows, table.holds, [p.grad for p in table.holds[0]]))
         if profiler.ACTIVE is not None:
             profiler.note("adamw_multi_step", "hbm", float(self._bytes))
         call("bts_adamw_multi_step", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, rows.data_ptr(), len(self.param_groups), hyper,

@@ -301,6 +301,62 @@ def test_on_a_stream_of_its_own():
     assert torch.equal(got, want)
 
 
+def test_two_threads_at_once():
+    """Two host threads, a stream each, forward and backward: every result is the one that a thread alone gets."""
+    import threading
+    cases = [make(3001, 96, torch.float32, 41), make(777, 2208, torch.bfloat16, 43)]
+    want, got, errors = [], [[], []], []
+    for x, w, b, dy in cases:
+        y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+        want.append((y,) + ops.layer_norm_bwd(dy, x, stats, w))
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            x, w, b, dy = (t.detach().clone().requires_grad_(k < 3) for k, t in enumerate(cases[i]))
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    y = layer_norm(x, w, b)
+                    got[i] = (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+            s.synchronize()
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not errors, errors
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_offsets_beyond_32_bits():
+    """2^31 + 6400 elements: the last rows come out like those of a short tensor, and the sums count every row."""
+    C, tail = 64, 100
+    M = 2 ** 31 // C + tail
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of free device memory")
+    gen = torch.Generator(device=DEV).manual_seed(47)
+    x = torch.zeros(M, C, dtype=torch.bfloat16, device=DEV)
+    x[-tail:] = torch.randn(tail, C, generator=gen, device=DEV).to(torch.bfloat16)
+    w, b = torch.rand(C, generator=gen, device=DEV) + 0.5, torch.randn(C, generator=gen, device=DEV)
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    short, sstats = ops.layer_norm_fwd(x[-tail:], w, b, 1e-5, want_stats=True)
+    assert torch.equal(y[-tail:], short) and torch.equal(stats[:, -tail:], sstats) and torch.equal(y[:3], b.to(torch.bfloat16).expand(3, C))
+    dy = y.zero_()
+    dy[-tail:] = torch.randn(tail, C, generator=gen, device=DEV).to(torch.bfloat16)
+    dy[0] = 1.0                                                             # a constant row: xh = 0, adds to the bias's gradient only
+    dx, dw, db = ops.layer_norm_bwd(dy, x, stats, w)
+    sdx, _, _ = ops.layer_norm_bwd(dy[-tail:], x[-tail:], sstats, w)
+    assert torch.equal(dx[-tail:], sdx) and (dx[1000:2000] == 0).all()
+    r = plain(x[-tail:], w, b, 1e-5, dy[-tail:])
+    within(dw, r["dw"], r["tol_dw"], "dweight")
+    within(db - 1.0, r["db"], r["tol_db"] + 200 * U, "dbias")
+
+
 def test_refusals_on_the_device():
     x, w, b, dy = make(8, 16, torch.float32, 37)
     for args in ((x.half(), w, b), (x.double(), w, b), (x, w[:15], b), (x, w.bfloat16(), b), (x, w.cpu(), b), (x, w, b[:1]),

@@ -255,7 +255,7 @@ def test_gradients_that_come_and_go():
     opt = optimizer(ps, 2, state_bits=8, max_grad_norm=1.0)
     assert opt.grad_norm is None
     opt.step()                                                              # no gradient at all: only the step count moves
-    assert opt.device_steps() == [1.0, 1.0] and not opt.state
+    assert opt.device_steps() == [1.0, 1.0] and not opt.state and opt.grad_norm.item() == 0.0
     feed(ps[:2], 1)
     check_step(opt)
     feed(ps, 2)
@@ -392,6 +392,26 @@ def test_captured_steps_replay(bits):
     oa.step()
     ob.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+def test_a_graph_outlives_what_it_was_captured_with():
+    """After the gradients are gone and a checkpoint is loaded, a replay still writes its own states and nothing else."""
+    ps = tensors([9000, 333], torch.float32, 37)
+    opt = optimizer(ps, 1, state_bits=8, max_grad_norm=0.5)
+    feed(ps, 1)
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step(prepared=True)
+    sd = copy.deepcopy(opt.state_dict())
+    opt.zero_grad(set_to_none=True)
+    opt.load_state_dict(sd)
+    fence = [torch.full((9000,), 3.0, device=DEV) for _ in range(64)]       # takes what the allocator has free
+    before = [t.clone() for t in opt.moments(flat=True)]
+    g.replay()
+    torch.cuda.synchronize()
+    assert all((t == 3.0).all() for t in fence)
+    assert all(torch.equal(a, b) for a, b in zip(before, opt.moments(flat=True))) and opt.device_steps() == [1.0, 1.0]
 
 
 def test_steps_on_several_streams():
