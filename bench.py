@@ -790,7 +790,7 @@ def main():
     own_opt = args.optimizer in ("bts", "bts8")
     if own_opt:
         from bts_amd.optim import FusedAdamW
-        opt = FusedAdamW(groups, lr=1e-4, eps=1e-3, state_bits=8 if args.optimizer == "bts8" else 32)
+        opt = FusedAdamW(groups, lr=1e-4, eps=1e-3, state_bits=8 if args.optimizer == "bts8" else None)
     else:
         opt = torch.optim.AdamW(groups, lr=lr_t if use_graph else 1e-4, eps=1e-3, fused=True, capturable=use_graph)
     crit = silog_loss(0.85)

@@ -20,8 +20,10 @@ whose per-parameter steps differ inside a group instead of silently rewriting th
 Gradients must keep their storage between steps (call ``zero_grad(set_to_none=False)``, the default here):
 the device pointer tables are rebuilt only when a pointer changes.
 
-Three options beyond that, all on `bts_adamw_multi_step` (csrc/adamw.hip; one update launch for ALL groups):
+Options beyond that, all on `bts_adamw_multi_step` (csrc/adamw.hip; one update launch for ALL groups):
 
+* ``state_bits=32``: f32 moments as without it, every constant formed in 64 bits.  (`bts_adamw_step`, which f32 parameters take when no option
+  is given, forms 1 - beta2 in f32: its exp_avg_sq is 4.7e-5 of itself larger for beta2 = 0.999, and bias_c2 with it, so the updates agree.)
 * ``state_bits=8``: the moments of parameters with at least ``min_8bit_size`` elements are held as 8-bit codes, 256 elements (in the
   parameter's memory order) to a power of two: 2 bytes of state per element instead of 8, read and written once per step.  Codes and
   scales are ``state[p]['exp_avg_codes' / 'exp_avg_scales' / 'exp_avg_sq_codes' / 'exp_avg_sq_scales']``; ``moments()`` gives the values that
@@ -115,15 +117,15 @@ class _Table:
 
 
 class FusedAdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None, min_8bit_size=4096):
-        if state_bits not in (8, 32):
-            raise BtsAmdError("FusedAdamW: state_bits must be 8 or 32, got %r" % (state_bits,))
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=None, max_grad_norm=None, min_8bit_size=4096):
+        if state_bits not in (8, 32, None):
+            raise BtsAmdError("FusedAdamW: state_bits must be 8, 32 or None, got %r" % (state_bits,))
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise BtsAmdError("FusedAdamW: max_grad_norm must be positive (or None), got %r" % (max_grad_norm,))
         if int(min_8bit_size) != min_8bit_size or min_8bit_size < 1:
             raise BtsAmdError("FusedAdamW: min_8bit_size must be a positive whole number, got %r" % (min_8bit_size,))
-        self._options = (state_bits, int(min_8bit_size), None if max_grad_norm is None else float(max_grad_norm))
-        self._multi = state_bits == 8 or max_grad_norm is not None
+        self._options = (state_bits or 32, int(min_8bit_size), None if max_grad_norm is None else float(max_grad_norm))
+        self._multi = state_bits is not None or max_grad_norm is not None
         self._forget()
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)

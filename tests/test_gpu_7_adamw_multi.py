@@ -87,10 +87,9 @@ def feed(ps, seed, scale=1.0):
             p.grad.copy_(g)
 
 
-# f32 parameters with 32-bit states and no clipping stay with bts_adamw_step, whose 1 - beta2 is formed in f32 (0.00100004673: v is
-# 4.7e-5 larger, and bias_c2 with it) and whose results are kept: tests/test_gpu_4_model.py holds it to torch.optim.AdamW
-@pytest.mark.parametrize("bits,least,dtype,clip", [(b, n, d, c) for b, n in ((8, 4096), (8, 1), (32, 4096)) for d in (torch.float32, torch.bfloat16)
-                                                   for c in (None, 0.5, float("inf")) if (b, d, c) != (32, torch.float32, None)])
+@pytest.mark.parametrize("clip", [None, 0.5, float("inf")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits,least", [(8, 4096), (8, 1), (32, 4096)])
 def test_steps_against_the_definition(bits, least, dtype, clip):
     ps = tensors(SIZES, dtype, 1)
     opt = optimizer(ps, 6, state_bits=bits, max_grad_norm=clip, min_8bit_size=least)
@@ -100,6 +99,22 @@ def test_steps_against_the_definition(bits, least, dtype, clip):
         check_step(opt)
     assert [("exp_avg_codes" in opt.state[p]) for p in ps] == [bits == 8 and n >= least for n in SIZES]
     assert opt.device_steps() == [4.0, 4.0]
+
+
+def test_without_options_the_step_stays_what_it_was():
+    """f32 parameters and no option: bts_adamw_step, whose 1 - beta2 is formed in f32 (0.00100004673).  bf16 parameters move to the
+    multi-tensor kernel by themselves."""
+    p = tensors([5000], torch.float32, 41)[0]
+    p.grad = torch.full_like(p, 2.0)
+    opt = FusedAdamW([p])
+    assert opt.state_bits == 32 and opt.max_grad_norm is None
+    opt.step()
+    assert (opt.state[p]["exp_avg_sq"] == (torch.tensor(1.0) - torch.tensor(0.999)).item() * 2.0 * 2.0).all()
+    q = tensors([5000], torch.bfloat16, 41)[0]
+    q.grad = torch.full_like(q, 2.0)
+    opt = FusedAdamW([q])
+    opt.step()
+    assert ((opt.state[q]["exp_avg_sq"] - 0.004).abs() <= 4 * U * 0.004).all()
 
 
 def test_mixed_types_in_one_step():

@@ -60,7 +60,7 @@ def test_modules_have_torch_parameters():
 def test_adamw_options_are_checked():
     from bts_amd.optim import FusedAdamW
     p = torch.nn.Parameter(torch.zeros(8))
-    for bad in (dict(state_bits=4), dict(state_bits=16), dict(max_grad_norm=0.0), dict(max_grad_norm=-1.0), dict(max_grad_norm=float("nan")),
+    for bad in (dict(state_bits=4), dict(state_bits=16), dict(state_bits=0), dict(max_grad_norm=0.0), dict(max_grad_norm=-1.0), dict(max_grad_norm=float("nan")),
                 dict(min_8bit_size=0), dict(min_8bit_size=1.5)):
         with pytest.raises(_lib.BtsAmdError):
             FusedAdamW([p], **bad)
