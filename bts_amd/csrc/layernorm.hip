@@ -157,30 +157,40 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Sum over the LANES lanes that hold a row.  LANES > 64: the whole block, through LDS (`red`: one float per wave).  Two sums of one
-// row use two sets, so one barrier per sum is enough: a set is written again only behind the barrier of the other.
+// Sum over the LANES lanes that hold a row.  LANES > 64: the whole block, through LDS (`red`: kRed<LANES> floats, one per wave, 0 where there
+// is no wave).  Two sums of one row use two sets, so one barrier per sum is enough: a set is written again only behind the barrier of
+// the other.
+template <int LANES>
+constexpr int kRed = LANES <= 128 ? 2 : LANES <= 256 ? 4 : LANES <= 512 ? 8 : 16;
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* red) {
     v = lane_sum<LANES < 64 ? LANES : 64>(v);
     if constexpr (LANES > 64) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         lds_barrier();
-        v = red[threadIdx.x & (LANES / 64 - 1)];
-        v = lane_sum<LANES / 64>(v);
+        v = lane_sum<kRed<LANES>>(red[threadIdx.x & (kRed<LANES> - 1)]);
     }
     return v;
+}
+template <int LANES>
+__device__ __forceinline__ void clear_sums(float* red) {                     // the entries that no wave writes
+    if constexpr (LANES > 64 && LANES != 64 * kRed<LANES>) {
+        if (threadIdx.x < 2 * kRed<LANES>) red[threadIdx.x] = 0.f;
+        __syncthreads();
+    }
 }
 
 // Bound by memory: 856064 x 96 bf16 63 us (5.2 TB/s; a large copy reaches 4.7-5.1), 8192 x 4096 f32 44 us (6.1, partly from the last-level
 // cache), 53504 x 128 f32 13.9 us, 418 x 512 bf16 3.3 us (launch and one latency).  Rows at odd addresses take two lines per vector:
-// 2000 x 8191 bf16 21.8 us, 3.0 TB/s.  Shared rows keep w and b in registers over the block's rows.
+// 2000 x 8191 bf16 18.3 us, 3.6 TB/s.  Shared rows keep w and b in registers over the block's rows.
 template <typename T, int LANES, int K, bool ODD>
 __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(const void* __restrict__ x, long xs, void* __restrict__ y, long ys,
                                                                                long M, int C, const float* __restrict__ w,
                                                                                const float* __restrict__ b, float eps,
                                                                                float* __restrict__ mean, float* __restrict__ rstd) {
     constexpr int V = T::kVec, RPB = LANES > 64 ? 1 : kThreads / LANES;
-    __shared__ float red[2][LANES > 64 ? LANES / 64 : 1];
+    __shared__ float red[2][kRed<LANES>];
+    clear_sums<LANES>(red[0]);
     const int lane = threadIdx.x % LANES;
     float wv[K][V], bv[K][V];
 #pragma unroll
@@ -226,8 +236,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(c
     }
 }
 
-// 856064 x 96 bf16 103 us (4.8 TB/s) + 5 us for the final sums, 8192 x 4096 bf16 41 + 7, 3344 x 2208 f32 18.2 + 4.5, 13376 x 512 bf16
-// 9.8 + 4.4, 418 x 512 bf16 3.7 + 3.0.
+// 856064 x 96 bf16 102 us (4.8 TB/s) + 5 us for the final sums, 8192 x 4096 bf16 35 + 5, 3344 x 2208 f32 18.5 + 4.0, 13376 x 512 bf16
+// 9.6 + 3.9, 2000 x 8191 bf16 28 + 6, 418 x 512 bf16 3.6 + 3.4.
 // Every block walks rows in steps of the grid and keeps the sums of dy xh and dy over its rows in registers; it writes one partial row
 // [2][C] (ws), ln_bwd_final_kernel adds the rows in a fixed order: no atomics, the gradients of the parameters are reproducible.
 template <typename T, int LANES, int K, bool ODD, bool PARAM>
@@ -236,7 +246,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(c
                                                                                const float* __restrict__ w, const float* __restrict__ mean,
                                                                                const float* __restrict__ rstd, float* __restrict__ ws) {
     constexpr int V = T::kVec, RPB = LANES > 64 ? 1 : kThreads / LANES;
-    __shared__ float red[2][LANES > 64 ? LANES / 64 : 1];
+    __shared__ float red[2][kRed<LANES>];
+    clear_sums<LANES>(red[0]);
     const int lane = threadIdx.x % LANES;
     float wv[K][V], dw[K][V], db[K][V];
 #pragma unroll
@@ -364,6 +375,8 @@ constexpr int kLnMaxC = 16384;
 // elements per lane, and 16 above 8192 elements.  Both sides, forward / backward with its sums, us: 856064 x 96 bf16 16 x 1: 70 / 106,
 // 8 x 2: 71 / 102, 4 x 3: 95 / 166; 400000 x 32 f32 8 x 1: 20.3 / 32.6, 2 x 4: 26.3 / 44.5; 13376 x 512 bf16 64 x 1: 7.3 / 15.8,
 // 16 x 4: 34 / 59; 16384 x 1024 bf16 64 x 2: 14.8 / 27.7, 128 x 1: 15.7 / 32.9; 8192 x 4096 bf16 512 x 1: 28.3 / 52, 256 x 2: 31.6 / 58.
+// bf16 rows of 3, 5 or 6 waves take just those (20000 x 1025: 29.8 / 46 -> 26.2 / 42, 30000 x 2049: 83 / 134 -> 78 / 105); wider rows, and f32
+// with its two vectors per lane, do not gain by it (4000 x 5120 bf16 22.3 -> 25.6 / 29.6, 8000 x 2208 f32 28.0 / 44 -> 29.1 / 53).
 static void ln_lanes(int V, int C, int& lanes, int& k) {
     const int nv = (C + V - 1) / V;
     int kmax = 1;
@@ -371,6 +384,7 @@ static void ln_lanes(int V, int C, int& lanes, int& k) {
     lanes = 1;
     while (lanes * kmax < nv) lanes *= 2;
     if (nv > 64 && C <= 1024) lanes = 64;
+    else if (nv > 64 && V == 8 && nv <= 384) lanes = (nv + 63) / 64 * 64;
     else if (nv > 64 && lanes < 256) lanes = 256;
     k = (nv + lanes - 1) / lanes;
 }
@@ -394,29 +408,19 @@ static bool ln_args(const void* x, int dtype, long M, int C) {
 
 }  // namespace
 
-#define LN_ODD(T, L, K, F) \
-    if (C % T::kVec) { F(T, L, K, true); } else { F(T, L, K, false); }
-#define LN_K2(T, L, F) \
-    if (p.k == 1) { LN_ODD(T, L, 1, F) } else { LN_ODD(T, L, 2, F) }
-#define LN_K4(T, L, F)                                         \
-    switch (p.k) {                                             \
-        case 1: LN_ODD(T, L, 1, F) break;                      \
-        case 2: LN_ODD(T, L, 2, F) break;                      \
-        case 3: LN_ODD(T, L, (T::kVec == 4 ? 3 : 2), F) break; \
-        default: LN_ODD(T, L, (T::kVec == 4 ? 4 : 2), F)       \
-    }
-#define LN_LANES(T, F)                      \
-    switch (p.lanes) {                      \
-        case 1: LN_ODD(T, 1, 1, F) break;   \
-        case 2: LN_ODD(T, 2, 1, F) break;   \
-        case 4: LN_ODD(T, 4, 1, F) break;   \
-        case 8: LN_ODD(T, 8, 1, F) break;   \
-        case 16: LN_ODD(T, 16, 1, F) break; \
-        case 32: LN_ODD(T, 32, 1, F) break; \
-        case 64: LN_K4(T, 64, F) break;     \
-        case 256: LN_K2(T, 256, F) break;   \
-        case 512: LN_K2(T, 512, F) break;   \
-        default: LN_K4(T, 1024, F)          \
+// every (lanes, vectors per lane) that ln_lanes gives for a type
+#define LN_CASE(T, L, K, F)                                            \
+    if (p.lanes == L && p.k == K) {                                    \
+        if (C % T::kVec) { F(T, L, K, true); } else { F(T, L, K, false); } \
+    } else
+#define LN_SHORT(T, F) LN_CASE(T, 1, 1, F) LN_CASE(T, 2, 1, F) LN_CASE(T, 4, 1, F) LN_CASE(T, 8, 1, F) LN_CASE(T, 16, 1, F) LN_CASE(T, 32, 1, F) LN_CASE(T, 64, 1, F) LN_CASE(T, 64, 2, F)
+#define LN_LAUNCH(F)                                                                                                                                \
+    if (dtype == BTS_F32) {                                                                                                                         \
+        LN_SHORT(F32, F) LN_CASE(F32, 64, 3, F) LN_CASE(F32, 64, 4, F) LN_CASE(F32, 256, 2, F) LN_CASE(F32, 512, 2, F)                              \
+        LN_CASE(F32, 1024, 2, F) LN_CASE(F32, 1024, 3, F) LN_CASE(F32, 1024, 4, F) return BTS_ERR_UNSUPPORTED;                                      \
+    } else {                                                                                                                                        \
+        LN_SHORT(BF16, F) LN_CASE(BF16, 192, 1, F) LN_CASE(BF16, 256, 1, F) LN_CASE(BF16, 320, 1, F) LN_CASE(BF16, 384, 1, F)                       \
+        LN_CASE(BF16, 512, 1, F) LN_CASE(BF16, 1024, 1, F) LN_CASE(BF16, 1024, 2, F) return BTS_ERR_UNSUPPORTED;                                    \
     }
 
 extern "C" int bts_layernorm_fwd(const void* x, int dtype, long x_stride, void* y, long y_stride, long M, int C, const float* w, const float* b,
@@ -429,7 +433,7 @@ extern "C" int bts_layernorm_fwd(const void* x, int dtype, long x_stride, void* 
 #define L_(T, LANES, K, ODD)                                                                                                                 \
     hipLaunchKernelGGL((ln_fwd_kernel<T, LANES, K, ODD>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, x, x_stride, y, \
                        y_stride, M, C, w, b, eps, mean, rstd)
-    if (dtype == BTS_F32) { LN_LANES(F32, L_) } else { LN_LANES(BF16, L_) }
+    LN_LAUNCH(L_)
 #undef L_
     BTS_LAUNCH_CHECK();
     return BTS_OK;
@@ -457,7 +461,7 @@ extern "C" int bts_layernorm_bwd(const void* dy, long dy_stride, const void* x, 
     else                                                                                                                             \
         hipLaunchKernelGGL((ln_bwd_kernel<T, LANES, K, ODD, false>), dim3((unsigned)p.blocks), dim3(LANES > 64 ? LANES : kThreads), 0, st, \
                            dy, dy_stride, x, x_stride, dx, dx_stride, M, C, w, mean, rstd, ws)
-    if (dtype == BTS_F32) { LN_LANES(F32, L_) } else { LN_LANES(BF16, L_) }
+    LN_LAUNCH(L_)
 #undef L_
     if (dw || db) hipLaunchKernelGGL(ln_bwd_final_kernel, dim3(ceil_div(2l * C, 32)), dim3(1024), 0, st, ws, (int)p.blocks, C, dw, db);
     BTS_LAUNCH_CHECK();

@@ -64,7 +64,7 @@ def make(M, C, dtype, seed, pad=0, offset=0):
 
 
 SHAPES = [(1, 1), (3, 2), (5, 3), (1, 7), (33, 8), (257, 16), (70, 17), (100, 33), (1000, 32), (513, 96), (66, 127), (9, 130), (418, 512), (31, 667), (40, 1024),
-          (17, 1025), (300, 2208), (7, 4097), (5, 8192), (3, 16384), (4, 16381), (20000, 24), (5000, 64)]
+          (17, 1025), (700, 1401), (33, 1537), (300, 2208), (19, 2049), (600, 2600), (7, 4097), (5, 8192), (3, 16384), (4, 16381), (20000, 24), (5000, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

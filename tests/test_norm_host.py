@@ -115,3 +115,26 @@ def test_the_written_down_8bit_forms():
             top = 448.0 if signed else 61440.0
             assert got.abs().max() <= top * 2.0 ** k and got.abs().max() > top * 2.0 ** (k - 1) * 0.96
         assert torch.equal(R.hold(y, signed)[0], y)
+
+
+def test_every_width_has_a_kernel():
+    """The rule for lanes and vectors (restated) covers every width of both types with a variant that the launcher lists, and of a row's
+    vectors per lane only the last may be missing: the kernels load the others without a check."""
+    src = open(_lib.os.path.join(_lib._HERE, "csrc", "layernorm.hip")).read()
+    import re
+    short = set(re.findall(r"LN_CASE\(T, (\d+), (\d+), F\)", src))
+    have = {t: {(int(a), int(b)) for a, b in short | set(re.findall(r"LN_CASE\(%s, (\d+), (\d+), F\)" % t, src))} for t in ("F32", "BF16")}
+    for t, vec in (("F32", 4), ("BF16", 8)):
+        seen = set()
+        for c in range(1, ops.LN_MAX_C + 1):
+            nv = -(-c // vec)
+            most = 1 if nv <= 64 else (16 if c <= 1024 or c > 8192 else 8) // vec
+            lanes = 1
+            while lanes * most < nv:
+                lanes *= 2
+            if nv > 64:
+                lanes = 64 if c <= 1024 else -(-nv // 64) * 64 if vec == 8 and nv <= 384 else max(lanes, 256)
+            k = -(-nv // lanes)
+            assert (lanes, k) in have[t] and lanes * k >= nv > lanes * (k - 1), (t, c, lanes, k)
+            seen.add((lanes, k))
+        assert seen == have[t]                       # and every listed variant is some width's
