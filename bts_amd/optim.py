@@ -41,7 +41,7 @@ captured with: capture again after ``load_state_dict`` or ``add_param_group``.
 import ctypes as C
 import itertools
 import math
-from operator import attrgetter
+from operator import attrgetter, is_
 
 import numpy as np
 import torch
@@ -383,19 +383,17 @@ class FusedAdamW(torch.optim.Optimizer):
     def _step_table(self):
         """The table of all parameters that have a gradient now.  What it was made from is compared every step: addresses and types of
         parameters and gradients and the gradients' strides; a gradient that moved costs one small upload, anything else a new table."""
-        ps, groups = [], []
-        for gi, g in enumerate(self.param_groups):
-            ps += g["params"]
-            groups += [gi] * len(g["params"])
+        ps = [p for g in self.param_groups for p in g["params"]]
+        lens, keep = [len(g["params"]) for g in self.param_groups], None
         gs = list(map(_grad, ps))
         if type(None) in set(map(type, gs)):
             keep = [i for i, g in enumerate(gs) if g is not None]
-            ps, groups, gs = [ps[i] for i in keep], [groups[i] for i in keep], [gs[i] for i in keep]
+            ps, gs = [ps[i] for i in keep], [gs[i] for i in keep]
         if not ps:
             return None
         gptr = list(map(_ptr, gs))
-        seen = (list(map(id, ps)), groups, list(map(_ptr, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
-        if self._plan is not None and seen == self._seen:
+        seen = (lens, keep, list(map(_ptr, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
+        if self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])):
             if gptr == self._gptr:
                 return self._plan
             self._no_capture("step", _RUN_FIRST)
@@ -403,6 +401,9 @@ class FusedAdamW(torch.optim.Optimizer):
             self._plan.upload(self._device())
             self._gptr = gptr
             return self._plan
+        groups = [gi for gi, n in enumerate(lens) for _ in range(n)]
+        if keep is not None:
+            groups = [groups[i] for i in keep]
         self._no_capture("step", _RUN_FIRST)
         self._check_parameters(ps)
         for p, g in zip(ps, gs):
