@@ -101,6 +101,24 @@ def test_steps_against_the_definition(bits, least, dtype, clip):
     assert opt.device_steps() == [4.0, 4.0]
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-11])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_small_eps_and_small_gradients(bits, eps):
+    """An eps that keeps nothing away from zero: gradients of 1e-14 .. 1e-8 (their squares are still normal f32 numbers) and the other
+    betas; lr 0 and no decay move nothing."""
+    gen = torch.Generator(device=DEV).manual_seed(43)
+    p = torch.randn(6000, generator=gen, device=DEV).requires_grad_(True)
+    opt = FusedAdamW([p], lr=1e-2, betas=(0.0, 0.5), eps=eps, weight_decay=0.0, state_bits=bits)
+    for it in range(3):
+        g = torch.randn(6000, generator=gen, device=DEV)
+        p.grad = torch.where(g.abs() < 1e-3, torch.full_like(g, 1e-3), g) * torch.logspace(-11, -8, 6000, device=DEV)
+        check_step(opt)
+    opt.param_groups[0]["lr"] = 0.0
+    was = p.detach().clone()
+    check_step(opt)
+    assert torch.equal(p, was)
+
+
 def test_without_options_the_step_stays_what_it_was():
     """f32 parameters and no option: bts_adamw_step, whose 1 - beta2 is formed in f32 (0.00100004673).  bf16 parameters move to the
     multi-tensor kernel by themselves."""
