@@ -26,10 +26,16 @@ def _rows(t):
 
 
 def _backward(ctx, dy):
-    x, weight, stats = ctx.saved_tensors
+    x, weight = ctx.saved_tensors
     need = ctx.needs_input_grad
     dy, (_, dys) = _rows(dy)
-    return (*ops.layer_norm_bwd_unchecked(dy, dys, x, ctx.rows, stats, weight, need[0], need[1], need[2]), None)
+    if x.stride() == ctx.strides and x.shape == dy.shape and x.dtype == dy.dtype and (
+            weight is None or weight.dtype == torch.float32 and weight.is_contiguous() and weight.numel() == x.shape[-1]):
+        return (*ops.layer_norm_bwd_unchecked(dy, dys, x, ctx.rows, ctx.stats, weight, need[0], need[1], need[2]), None)
+    # Saved-tensor hooks gave back other tensors than were saved (save_on_cpu: a slice of a wider buffer comes back dense): their own
+    # layout counts, and what is not the saved values' shape, type and device is refused.
+    weight = weight if weight is None else weight.contiguous()
+    return (*ops.layer_norm_bwd(dy, _rows(x)[0], ctx.stats, weight, need[0], need[1], need[2]), None)
 
 
 _backward_once = once_differentiable(_backward)
@@ -40,8 +46,8 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         x, rows = _rows(x)
         y, stats = ops.layer_norm_fwd_rows(x, rows, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.rows = rows
+        ctx.save_for_backward(x, weight)
+        ctx.rows, ctx.strides, ctx.stats = rows, x.stride(), stats           # (nobody else has the statistics: not for hooks to change)
         return y
 
     @staticmethod

@@ -377,3 +377,16 @@ def test_refusals_on_the_device():
     (g,) = torch.autograd.grad(layer_norm(x, w, b).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensor_hooks_may_change_the_layout(dtype):
+    """save_on_cpu gives a channel slice back as a dense tensor: the gradients are those of the pass without hooks."""
+    x, w, b, dy = make(401, 667, dtype, 53, pad=5)
+    x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+    want = torch.autograd.grad(layer_norm(x, w, b), (x, w, b), dy)
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True), torch.autograd.graph.saved_tensors_hooks(torch.clone, lambda t: t)):
+        with hooks:
+            y = layer_norm(x, w, b)
+        got = torch.autograd.grad(y, (x, w, b), dy)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))

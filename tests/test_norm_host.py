@@ -138,3 +138,54 @@ def test_every_width_has_a_kernel():
             assert (lanes, k) in have[t] and lanes * k >= nv > lanes * (k - 1), (t, c, lanes, k)
             seen.add((lanes, k))
         assert seen == have[t]                       # and every listed variant is some width's
+
+
+@pytest.fixture
+def stubbed_norm(monkeypatch):
+    """layer_norm on CPU tensors: the launches are recorded, nothing is computed.  -> list of (name, x, its rows and stride) per launch."""
+    seen = []
+
+    def fwd(x, rows, weight, bias, eps, want_stats):
+        seen.append(("fwd", x, rows))
+        y = torch.zeros(x.shape, dtype=x.dtype)
+        return (y, torch.zeros(2, rows[0])) if want_stats else y
+
+    def bwd(dy, dys, x, rows, stats, weight, want_dx, want_dweight, want_dbias):
+        seen.append(("bwd", x, rows))
+        assert x.stride()[-1] == 1 and ops.row_stride(x) == rows and ops.row_stride(dy)[1] == dys and stats.shape == (2, rows[0])
+        return tuple(torch.zeros(s, dtype=t) if w else None for w, s, t in zip(
+            (want_dx, want_dweight, want_dbias), (x.shape, x.shape[-1:], x.shape[-1:]), (x.dtype, torch.float32, torch.float32)))
+    monkeypatch.setattr(ops, "layer_norm_fwd_rows", fwd)
+    monkeypatch.setattr(ops, "layer_norm_bwd_unchecked", bwd)
+    monkeypatch.setattr(_lib, "require_gpu", lambda t: None)
+    monkeypatch.setattr(ops, "current_device", lambda: -1)
+    return seen
+
+
+def test_backward_goes_by_the_layout_of_what_hooks_give_back(stubbed_norm):
+    """A saved-tensor hook may give a strided input back dense: the launch must not walk it with the stride of the tensor that was saved
+    (for 401 rows of 667 in 672 columns it would end 2000 elements behind it)."""
+    w, b = torch.ones(667, requires_grad=True), torch.zeros(667, requires_grad=True)
+    x = torch.randn(401, 672)[:, :667].requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+        layer_norm(x, w, b).sum().backward()
+    assert stubbed_norm[-1][2] == (401, 672)
+    for pack in (torch.clone, lambda t: t.contiguous().clone()):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            layer_norm(x, w, b).sum().backward()
+        assert stubbed_norm[-1][0] == "bwd" and stubbed_norm[-1][1].shape == (401, 667) and stubbed_norm[-1][2] == (401, 667)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t()):     # another order in memory
+        layer_norm(x, w, b).sum().backward()
+    assert stubbed_norm[-1][2] == (401, 667)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.bfloat16(), lambda t: t[..., :-1], lambda t: t.double()])
+def test_backward_refuses_other_values_than_were_saved(stubbed_norm, change):
+    x = torch.randn(8, 16, requires_grad=True)
+    for w, dtype in ((None, torch.float32), (torch.ones(16, requires_grad=True), torch.bfloat16)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            y = layer_norm(x.to(dtype), w)
+        n = len(stubbed_norm)
+        with pytest.raises(_lib.BtsAmdError):
+            y.sum().backward()
+        assert len(stubbed_norm) == n
