@@ -56,7 +56,7 @@ _BF16, _8BIT = 1, 2
 _RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("m_scale", "u8"), ("v_scale", "u8"), ("n", "i8"), ("group", "i4"), ("flags", "i4")])
 _RUN_FIRST = "run one step with the same parameters and gradients (zero_grad(set_to_none=False) keeps them)"
 _CODES = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")
-_ptr, _stride, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, attrgetter("grad"), attrgetter("dtype")
+_ptr, _stride, _numel, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, torch.Tensor.numel, attrgetter("grad"), attrgetter("dtype")
 
 
 def _dense(t):
@@ -370,7 +370,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 if not (a.dtype == b.dtype == torch.uint8 and sa.dtype == sb.dtype == torch.float32 and a.is_contiguous() and b.is_contiguous()
                         and a.data_ptr() % 4 == 0 and b.data_ptr() % 4 == 0 and a.numel() == b.numel() == n
                         and sa.numel() == sb.numel() == -(-n // _BLOCK) and _room(a) >= sa.numel() * _BLOCK and _room(b) >= sa.numel() * _BLOCK):
-                    raise BtsAmdError("FusedAdamW: the 8-bit state of a parameter was replaced by something else")
+                    raise BtsAmdError("FusedAdamW: the 8-bit state of a parameter of %d elements was replaced by something else, or is one of %d elements" % (n, a.numel()))
                 rows.append((p.data_ptr(), 0, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), n, gi, flags | _8BIT))
             else:
                 a, b = st["exp_avg"], st["exp_avg_sq"]
@@ -381,34 +381,37 @@ class FusedAdamW(torch.optim.Optimizer):
         return np.array(rows, dtype=_RECORD)
 
     def _step_table(self):
-        """The table of all parameters that have a gradient now.  What it was made from is compared every step: addresses and types of
+        """The table of all parameters that have a gradient now.  What it was made from is compared every step: addresses, sizes and types of
         parameters and gradients and the gradients' strides; a gradient that moved costs one small upload, anything else a new table."""
         ps = [p for g in self.param_groups for p in g["params"]]
         lens, keep = [len(g["params"]) for g in self.param_groups], None
         gs = list(map(_grad, ps))
-        if type(None) in set(map(type, gs)):
+        try:
+            gptr = list(map(_ptr, gs))
+        except TypeError:                               # some have none
             keep = [i for i, g in enumerate(gs) if g is not None]
             ps, gs = [ps[i] for i in keep], [gs[i] for i in keep]
+            gptr = list(map(_ptr, gs))
         if not ps:
             return None
-        gptr = list(map(_ptr, gs))
-        seen = (lens, keep, list(map(_ptr, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
+        seen = (lens, keep, list(map(_ptr, ps)), list(map(_numel, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
         if self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])):
             if gptr == self._gptr:
                 return self._plan
-            self._no_capture("step", _RUN_FIRST)
-            self._plan.host["g"] = gptr
-            self._plan.upload(self._device())
-            self._gptr = gptr
-            return self._plan
+            if list(map(_numel, gs)) == seen[3]:
+                self._no_capture("step", _RUN_FIRST)
+                self._plan.host["g"] = gptr
+                self._plan.upload(self._device())
+                self._gptr = gptr
+                return self._plan
         groups = [gi for gi, n in enumerate(lens) for _ in range(n)]
         if keep is not None:
             groups = [groups[i] for i in keep]
         self._no_capture("step", _RUN_FIRST)
         self._check_parameters(ps)
         for p, g in zip(ps, gs):
-            if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or not _same_layout(g, p):
-                raise BtsAmdError("FusedAdamW needs gradients of the parameter's type and layout on its device: parameter %s %s %s, gradient %s %s %s" % (
+            if g.layout != torch.strided or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape or not _same_layout(g, p):
+                raise BtsAmdError("FusedAdamW needs gradients of the parameter's type, shape and layout on its device: parameter %s %s %s, gradient %s %s %s" % (
                     tuple(p.shape), p.dtype, p.stride(), tuple(g.shape), g.dtype, g.stride() if g.layout == torch.strided else g.layout))
         fresh = [p for p in ps if not self.state.get(p)]
         if fresh:
@@ -429,10 +432,10 @@ class FusedAdamW(torch.optim.Optimizer):
     def _state_table(self):
         """The table of all parameters that have a state, for bts_adamw_multi_moments, and where each begins in flat moments."""
         ps = [p for g in self.param_groups for p in g["params"]]
-        key = (list(map(id, ps)), len(self.state))
+        sizes = list(map(_numel, ps))
+        key = (list(map(id, ps)), sizes, len(self.state))
         if self._state_plan is None or self._state_plan["key"] != key:
             self._no_capture("moments", "call moments() once")
-            sizes = [p.numel() for p in ps]
             offs = [0] + list(itertools.accumulate(sizes))
             have = [i for i, p in enumerate(ps) if self.state.get(p)]
             hp = [ps[i] for i in have]

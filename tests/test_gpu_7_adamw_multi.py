@@ -572,3 +572,23 @@ def test_normalised_head_trained_with_clipped_8bit_steps():
             assert (p.grad.double().cpu() - r.grad).abs().max() <= 200 * U * r.grad.abs().max() + 1e-9
         check_step(opt)
     assert "exp_avg_codes" in opt.state[conv.weight] and "exp_avg" in opt.state[norm.weight]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_parameter_that_shrinks_in_place_is_refused(bits):
+    p = tensors([9000], torch.float32, 47)[0]
+    opt = optimizer([p], None, state_bits=bits)
+    feed([p], 1)
+    check_step(opt)
+    whole = p.detach()
+    was = whole.clone()
+    p.data = p.data[:5000]
+    p.grad = torch.ones(5000, device=DEV)
+    for use in (opt.step, opt.moments, opt.state_dict):
+        with pytest.raises(BtsAmdError):
+            use()
+    assert torch.equal(whole, was)
+    p.data = whole
+    p.grad = None
+    feed([p], 2)
+    check_step(opt)

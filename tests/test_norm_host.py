@@ -189,3 +189,60 @@ def test_backward_refuses_other_values_than_were_saved(stubbed_norm, change):
         with pytest.raises(_lib.BtsAmdError):
             y.sum().backward()
         assert len(stubbed_norm) == n
+
+
+@pytest.fixture
+def stubbed_adamw(monkeypatch):
+    """FusedAdamW with options on CPU tensors: no launch happens, each is recorded as (name, records of its table, chunks of its table)."""
+    from bts_amd import optim
+    launches, empty, tables = [], torch.empty, {}
+
+    def table(self, *a):
+        init(self, *a)
+        tables[self.chunks.data_ptr()] = self
+    init = optim._Table.__init__
+
+    def call(name, *args):
+        t = tables.get(args[1]) if name in ("bts_adamw_multi_step", "bts_adamw_multi_moments") else None
+        launches.append((name, None, None) if t is None else (name, t.records.numpy().copy().view(optim._RECORD), t.chunks.numpy().copy()))
+        return 16384 if name == "bts_adamw_multi_workspace_bytes" else 0
+    for name, value in (("call", call), ("require_gpu", lambda t: None), ("current_device", lambda: None), ("raw_stream", lambda: 0)):
+        monkeypatch.setattr(optim, name, value)
+    monkeypatch.setattr(optim._Table, "__init__", table)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch, "empty", lambda *a, pin_memory=False, **kw: empty(*a, **kw))
+    return launches
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_sees_a_parameter_that_shrinks_in_place(stubbed_adamw, bits):
+    """p.data = p.data[:k] keeps the address and, for a vector, the stride: a launch with the old length would read behind the new gradient."""
+    from bts_amd.optim import FusedAdamW
+    p, q = torch.nn.Parameter(torch.zeros(9000)), torch.nn.Parameter(torch.zeros(50))
+    opt = FusedAdamW([p, q], state_bits=bits)
+    p.grad, q.grad = torch.zeros(9000), torch.zeros(50)
+    opt.step()
+    assert stubbed_adamw[-1][1]["n"].tolist() == [9000, 50]
+    p.grad = torch.zeros(9000)                                  # a gradient elsewhere: the same table, its address in it
+    opt.step()
+    assert stubbed_adamw[-1][1]["g"].tolist() == [p.grad.data_ptr(), q.grad.data_ptr()]
+    opt.moments()
+    n = len(stubbed_adamw)
+    p.data = p.data[:5000]
+    for grad in (torch.zeros(5000), None):                      # a new gradient; none set anew: the old one, of 9000 elements
+        if grad is not None:
+            p.grad = grad
+        else:
+            p.data = p.data[:4500]
+        for use in (opt.step, opt.step, opt.moments):           # its state is one of 9000 elements: refused, again and again
+            with pytest.raises(_lib.BtsAmdError):
+                use()
+    assert len(stubbed_adamw) == n
+    p.data, p.grad = torch.zeros(9000), torch.zeros(9000)
+    opt.step()
+    assert stubbed_adamw[-1][1]["n"].tolist() == [9000, 50]
+    n = len(stubbed_adamw)
+    p.grad.data = torch.zeros(8000)                             # a gradient that is not the parameter's any more
+    with pytest.raises(_lib.BtsAmdError):
+        opt.step()
+    assert len(stubbed_adamw) == n
