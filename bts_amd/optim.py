@@ -98,22 +98,30 @@ class _Table:
         self.holds = self.offsets = None        # what must live as long as the addresses; begin of each tensor in flat moments
         self.chunks = torch.from_numpy(chunks).to(device)
         self.records = torch.from_numpy(records.view(np.uint8)).to(device)
-        self.made_on = raw_stream()
+        self.records_on, self.used_on = raw_stream(), set()
 
     def upload(self, device):
         """A new device copy of the records, without waiting for it: launches in flight may still read the old one."""
         pinned = torch.empty(self.host.nbytes, dtype=torch.uint8, pin_memory=True)
         pinned.numpy()[:] = self.host.view(np.uint8)
         self.records = pinned.to(device, non_blocking=True)
-        self.made_on = raw_stream()
+        self.records_on = raw_stream()
 
-    def use(self):
-        """Called before a launch on the current stream: memory that the allocator gave to another one must outlive this one's work."""
-        if raw_stream() != self.made_on:
-            cur = torch.cuda.current_stream()
-            for t in (self.records, self.chunks, self.offsets):
-                if t is not None:
-                    t.record_stream(cur)
+    def use(self, stream):
+        """Called before a launch on `stream`, the current one: memory that the allocator gave to another one must outlive this one's work
+        -- the tables, and the states that the launch writes, also where the optimizer drops them while it runs."""
+        if stream not in self.used_on:
+            self.used_on.add(stream)
+            _record([self.chunks, self.offsets] + list({t.untyped_storage().data_ptr(): t for t in self.holds[1] if t.numel()}.values()))
+        if stream != self.records_on:
+            _record([self.records])
+
+
+def _record(ts):
+    cur = torch.cuda.current_stream()
+    for t in ts:
+        if t is not None and t.numel():
+            t.record_stream(cur)            # (nothing to do, and nothing done, for memory of the current stream)
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -141,6 +149,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._seen = self._plan = self._state_plan = None
         self._kept = []             # what captured graphs refer to
         self._scratch = self._norm = None
+        self._used_on = set()       # streams that _hyper, _scratch and _norm are recorded for
 
     def __getstate__(self):         # copies and pickles: states with their step counts, nothing that holds addresses
         self._refresh_steps()
@@ -191,6 +200,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def _rows(self):
         """The device rows, created on first use from the groups' hyper-parameters and recorded state."""
         if self._hyper is None:
+            self._used_on = set()
             if self._multi:
                 rows = np.zeros((len(self.param_groups) + 1, _WIDE_ROW))
                 for r, g in zip(rows, self.param_groups):
@@ -204,6 +214,16 @@ class FusedAdamW(torch.optim.Optimizer):
                 rows.append([float(g["lr"]), 1.0, 1.0, self._group_step_from_state(g), float(b1), float(b2), 0.0, 0.0])
             self._hyper = torch.tensor(rows, dtype=torch.float32).to(self._device())
         return self._hyper
+
+    def _launch_on(self, table=None):
+        """The current stream, for a launch that works on the rows, and on what `table` says."""
+        stream = raw_stream()
+        if stream not in self._used_on:
+            self._used_on.add(stream)
+            _record([self._hyper, self._scratch, self._norm])
+        if table is not None:
+            table.use(stream)
+        return stream
 
     def _host_hyper(self, lrs=None):
         """The groups' hyper-parameters as bts_adamw_multi_step takes them from the host."""
@@ -222,7 +242,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 return self.prepare_step(lrs)
         rows = self._rows()
         if self._multi:
-            call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), self._host_hyper(lrs), raw_stream())
+            call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), self._host_hyper(lrs), self._launch_on())
             return
         vals = [float(g["lr"] if lrs is None else lrs[gi]) for gi, g in enumerate(self.param_groups)]
         rows[:, 0].copy_(torch.tensor(vals, dtype=torch.float32))
@@ -457,13 +477,13 @@ class FusedAdamW(torch.optim.Optimizer):
         table, total = plan["table"], plan["total"]
         m, v = ((torch.empty if plan["all"] else torch.zeros)(total, dtype=torch.float32, device=self._device()) for _ in range(2))
         if table.n_chunks:
-            table.use()
+            stream = self._launch_on(table)
             if torch.cuda.is_current_stream_capturing():
                 self._kept.append((table.records, table.chunks, table.offsets, table.holds))
             if profiler.ACTIVE is not None:
                 profiler.note("adamw_moments", "hbm", 10.0 * total)
             call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
-                 m.data_ptr(), v.data_ptr(), 0, raw_stream())
+                 m.data_ptr(), v.data_ptr(), 0, stream)
         if flat:
             return m, v
         return [(_like(m, plan["at"][id(p)], p), _like(v, plan["at"][id(p)], p)) for g in self.param_groups for p in g["params"]]
@@ -477,21 +497,22 @@ class FusedAdamW(torch.optim.Optimizer):
             if self._norm is None:
                 self._norm = torch.zeros(1, dtype=torch.float32, device=self._device())
                 self._scratch = torch.empty(call("bts_adamw_multi_workspace_bytes") // 8, dtype=torch.float64, device=self._device())
+                self._used_on = set()
             norm = self._norm.data_ptr()
+        stream = self._launch_on(table)
         if table is None or not table.n_chunks:         # no gradient at all: the step count goes on, as bts_adamw_advance does
             if hyper is not None:
-                call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), hyper, raw_stream())
+                call("bts_adamw_multi_set", rows.data_ptr(), len(self.param_groups), hyper, stream)
             rows[:len(self.param_groups), 3] += 1
             if norm is not None:
                 self._norm.zero_()
             return
-        table.use()
         if torch.cuda.is_current_stream_capturing():
             self._kept.append((table.records, table.chunks, rows, table.holds, [p.grad for p in table.holds[0]]))
         if profiler.ACTIVE is not None:
             profiler.note("adamw_multi_step", "hbm", float(self._bytes))
         call("bts_adamw_multi_step", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, rows.data_ptr(), len(self.param_groups), hyper,
-             self._scratch.data_ptr() if norm is not None else None, norm, raw_stream())
+             self._scratch.data_ptr() if norm is not None else None, norm, stream)
         # parameters were updated through raw pointers: tell autograd / any version-keyed cache
         torch.autograd.graph.increment_version(table.holds[0])
 

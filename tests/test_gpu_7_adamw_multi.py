@@ -592,3 +592,29 @@ def test_a_parameter_that_shrinks_in_place_is_refused(bits):
     p.grad = None
     feed([p], 2)
     check_step(opt)
+
+
+def test_memory_dropped_while_another_stream_steps():
+    """Tables, rows and states that were made on one stream and are dropped there while a step on another one still has to run: nobody else
+    gets them before."""
+    ps, qs = tensors([9000, 333], torch.float32, 59), tensors([9000, 333], torch.float32, 59)
+    oa, ob = optimizer(ps, 1, state_bits=8, max_grad_norm=0.5), optimizer(qs, 1, state_bits=8, max_grad_norm=0.5)
+    for o, ts in ((oa, ps), (ob, qs)):
+        feed(ts, 1)
+        o.step()
+    sd = copy.deepcopy(oa.state_dict())
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for p in ps:
+            p.grad = None
+        feed(ps, 2)                                                         # other gradients: new records on this stream, the chunks stay
+        torch.cuda._sleep(100000000)
+        oa.step()
+    oa.load_state_dict(sd)                                                  # drops the table, the rows and the states
+    fence = [torch.full((n,), 3.0, device=DEV) for n in (4, 40, 300, 1000, 9000) * 40]
+    torch.cuda.synchronize()
+    assert all((t == 3.0).all() for t in fence)
+    feed(qs, 2)
+    ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and oa.device_steps() == [1.0, 1.0]

@@ -210,6 +210,8 @@ def stubbed_adamw(monkeypatch):
         monkeypatch.setattr(optim, name, value)
     monkeypatch.setattr(optim._Table, "__init__", table)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: 0)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, s: None)
     monkeypatch.setattr(torch, "empty", lambda *a, pin_memory=False, **kw: empty(*a, **kw))
     return launches
 
@@ -246,3 +248,43 @@ def test_adamw_sees_a_parameter_that_shrinks_in_place(stubbed_adamw, bits):
     with pytest.raises(_lib.BtsAmdError):
         opt.step()
     assert len(stubbed_adamw) == n
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_memory_outlives_the_work_of_every_stream(stubbed_adamw, monkeypatch, bits):
+    """Table made on one stream, used on others: everything that a launch reads and writes is recorded for the launch's stream (recording
+    memory for its own stream does nothing), also after a gradient moved and the records alone were made anew."""
+    from bts_amd import optim
+    now, recorded = [0], set()
+    monkeypatch.setattr(optim, "raw_stream", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: now[0])
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, s: recorded.add((self.untyped_storage().data_ptr(), s)))
+    p, q = torch.nn.Parameter(torch.zeros(9000)), torch.nn.Parameter(torch.zeros(50))
+    opt = optim.FusedAdamW([p, q], state_bits=bits, max_grad_norm=1.0)
+    p.grad, q.grad = torch.zeros(9000), torch.zeros(50)
+
+    def kept(*more):
+        own = [t for st in opt.state.values() for k, t in st.items() if k != "step"]
+        return {t.untyped_storage().data_ptr() for t in own + list(more) if t is not None}
+    opt.step()
+    opt.moments()
+    for stream in (1, 2):
+        now[0] = stream
+        recorded.clear()
+        p.grad = torch.zeros(9000)                              # a new copy of the records, made on this stream
+        opt.step()
+        mine = kept(opt._plan.chunks, opt._hyper, opt._norm, opt._scratch)
+        assert mine <= {t for t, s in recorded if s == stream}
+        opt.moments()
+        table = opt._state_plan["table"]
+        assert kept(table.chunks, table.records, table.offsets) <= {t for t, s in recorded if s == stream}
+    now[0] = 1                                                  # the records of the last upload belong to stream 2
+    recorded.clear()
+    opt.step()
+    assert (opt._plan.records.data_ptr(), 1) in recorded
+    opt._hyper = None                                           # new rows, used for the first time by prepare_step on stream 3
+    now[0] = 0
+    opt._rows()
+    now[0] = 3
+    opt.prepare_step()
+    assert (opt._hyper.data_ptr(), 3) in recorded
