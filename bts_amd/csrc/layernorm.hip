@@ -4,7 +4,8 @@
 //   h = dy w:  dx = r (h - mean(h) - xh mean(h xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // A row lives in the registers of LANES lanes (K vectors of 16 bytes each), so x (and dy) are read once: the mean first, then the
-// centred squares -- no E[x^2] - mu^2 cancellation.  Statistics, sums and parameters are f32; only x, y, dy, dx may be bf16.
+// centred squares -- no E[x^2] - mu^2 cancellation.  Where a row lies far from zero for its spread, the mean's own rounding is taken out
+// again.  Statistics, sums and parameters are f32; only x, y, dy, dx may be bf16.
 #include "common.h"
 
 namespace {
@@ -172,25 +173,34 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     }
     return v;
 }
-template <int LANES>
+template <int LANES, int SETS>
 __device__ __forceinline__ void clear_sums(float* red) {                     // the entries that no wave writes
     if constexpr (LANES > 64 && LANES != 64 * kRed<LANES>) {
-        if (threadIdx.x < 2 * kRed<LANES>) red[threadIdx.x] = 0.f;
+        if (threadIdx.x < SETS * kRed<LANES>) red[threadIdx.x] = 0.f;
         __syncthreads();
     }
 }
 
+// The mean of a row is off by its own rounding and the sum's, a few 2^-24 of |mu|; divided by the deviation that is nothing for most
+// rows and everything for a row of equal elements, where the deviation is sqrt(eps) (1000 in 7 columns: 0.019 instead of 0).  The
+// centred elements are small, so their mean says by how much it is off (divided by C, not multiplied by 1 / C: exact where all are
+// equal).  Rows with |mu| > 4 sqrt(var + eps) pay for it; what it would take out of the others is at most 5 times their sum's roundings.
+// us where no row / every row is one: 856064 x 96 bf16 63 / 84, 8192 x 4096 bf16 26 / 34, f32 43.5 / 45, 3344 x 2208 f32 12.6 / 15.9;
+// taken for every row regardless it costs rows near zero 71, 31, 44 and 14.3.
+constexpr float kFar = 16.f;
+
 // Bound by memory: 856064 x 96 bf16 63 us (5.2 TB/s; a large copy reaches 4.7-5.1), 8192 x 4096 f32 44 us (6.1, partly from the last-level
 // cache), 53504 x 128 f32 13.9 us, 418 x 512 bf16 3.3 us (launch and one latency).  Rows at odd addresses take two lines per vector:
 // 2000 x 8191 bf16 18.3 us, 3.6 TB/s.  Shared rows keep w and b in registers over the block's rows.
+// Rows of 1024 lanes are held to 64 registers where that spills nothing: two blocks a CU (2000 x 12288 bf16: 21 us, 26 at 68 registers).
 template <typename T, int LANES, int K, bool ODD>
-__global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(const void* __restrict__ x, long xs, void* __restrict__ y, long ys,
+__global__ __launch_bounds__(LANES > 64 ? LANES : kThreads, LANES == 1024 && !ODD ? 8 : 1) void ln_fwd_kernel(const void* __restrict__ x, long xs, void* __restrict__ y, long ys,
                                                                                long M, int C, const float* __restrict__ w,
                                                                                const float* __restrict__ b, float eps,
                                                                                float* __restrict__ mean, float* __restrict__ rstd) {
     constexpr int V = T::kVec, RPB = LANES > 64 ? 1 : kThreads / LANES;
-    __shared__ float red[2][kRed<LANES>];
-    clear_sums<LANES>(red[0]);
+    __shared__ float red[4][kRed<LANES>];
+    clear_sums<LANES, 4>(red[0]);
     const int lane = threadIdx.x % LANES;
     float wv[K][V], bv[K][V];
 #pragma unroll
@@ -211,7 +221,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(c
 #pragma unroll
             for (int e = 0; e < V; ++e) s += f[j][e];
         }
-        const float mu = row_sum<LANES>(s, red[0]) * inv;
+        float mu = row_sum<LANES>(s, red[0]) * inv;
         float q = 0.f;
 #pragma unroll
         for (int j = 0; j < K; ++j)
@@ -221,7 +231,26 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_fwd_kernel(c
                 f[j][e] = j < K - 1 || (lane + j * LANES) * V + (ODD ? e : 0) < C ? d : 0.f;
                 q += f[j][e] * f[j][e];
             }
-        const float rs = 1.f / sqrtf(row_sum<LANES>(q, red[1]) * inv + eps);
+        q = row_sum<LANES>(q, red[1]) * inv;
+        if (mu * mu > kFar * (q + eps)) {                                    // the same for all lanes of a row
+            float off = 0.f;
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) off += f[j][e];
+            off = row_sum<LANES>(off, red[2]) / (float)C;
+            mu += off;
+            q = 0.f;
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    f[j][e] -= off;
+                    if (j < K - 1 || (lane + j * LANES) * V + (ODD ? e : 0) < C) q += f[j][e] * f[j][e];
+                }
+            q = row_sum<LANES>(q, red[3]) * inv;
+        }
+        const float rs = 1.f / sqrtf(q + eps);
         if (mean && on && lane == 0) {
             mean[row] = mu;
             rstd[row] = rs;
@@ -247,7 +276,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(c
                                                                                const float* __restrict__ rstd, float* __restrict__ ws) {
     constexpr int V = T::kVec, RPB = LANES > 64 ? 1 : kThreads / LANES;
     __shared__ float red[2][kRed<LANES>];
-    clear_sums<LANES>(red[0]);
+    clear_sums<LANES, 2>(red[0]);
     const int lane = threadIdx.x % LANES;
     float wv[K][V], dw[K][V], db[K][V];
 #pragma unroll

@@ -390,3 +390,40 @@ def test_saved_tensor_hooks_may_change_the_layout(dtype):
             y = layer_norm(x, w, b)
         got = torch.autograd.grad(y, (x, w, b), dy)
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [1, 3, 7, 41, 200, 257, 667, 1025, 2208, 2900, 4097, 8191, 9001, 16384])
+def test_rows_of_equal_elements_are_centred_exactly(C, dtype):
+    """Variance 0, whatever the value and the width.  Far from zero (|mean| > 4 sqrt(eps)) y is the bias and the mean is the value, bit for
+    bit, and the weight's gradient is 0; below, and for the statistics of what is left there, the tolerances of any row hold."""
+    values = torch.tensor([3.25, 1000.0, 1000.1, 30000.0, -0.1, 1.0 / 3, 65504.0, -1e6, 2.0 ** 20 + 0.3, 0.0, 1e-30, 1e-3, -0.01], device=DEV).to(dtype)
+    M, far = values.numel(), 10
+    _, w, b, dy = make(M, C, dtype, 61)
+    x = values[:, None].expand(M, C).contiguous()
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    assert torch.equal(y[:far], b.to(dtype).expand(far, C)) and torch.equal(stats[0, :far], values[:far].float())
+    assert ((stats[1].double() * 1e-5 ** 0.5 - 1).abs() <= 4 * U).all()                # root, reciprocal, eps in f32
+    dx, dw, db = ops.layer_norm_bwd(dy, x, stats, w)
+    r = plain(x, w, b, 1e-5, dy)
+    within(y, r["y"], r["tol_y"], "y", HALF[dtype])
+    within(dx, r["dx"], r["tol_dx"], "dx", HALF[dtype])
+    within(db, r["db"], r["tol_db"], "dbias")
+    _, dw, _ = ops.layer_norm_bwd(dy[:far], x[:far], stats[:, :far].contiguous(), w)
+    assert (dw == 0).all()
+
+
+@pytest.mark.parametrize("C", [41, 667, 2208, 9001])
+def test_nearly_equal_elements_far_from_zero(C):
+    """Rows at 1000 whose elements differ in the last bits: the spread is 2^-13 of sqrt(eps) and less, and what the kernel centres is exact,
+    so the normalised values are good to a few roundings of their largest -- without the mean's own rounding, magnified."""
+    gen = torch.Generator(device=DEV).manual_seed(67)
+    steps = torch.randint(-3, 4, (50, C), generator=gen, device=DEV)
+    x = (1000.0 + steps.double() * 2.0 ** -14).float()
+    y, stats = ops.layer_norm_fwd(x, None, None, 1e-5, want_stats=True)
+    x64 = x.double()
+    xc = x64 - x64.mean(1, keepdim=True)
+    want = xc / (xc.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    # elements and mean are multiples of 2^-14 below 2^10: a difference of them is exact, but for the mean's correction, which adds up at
+    # most 42 times (u each) and is at most 43 u 1000 itself; root, reciprocal, product
+    assert ((y.double() - want).abs() <= 50 * U * (want.abs() + 43 * U * 1000 / 1e-5 ** 0.5)).all()
