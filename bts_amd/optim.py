@@ -76,13 +76,21 @@ def _room(t):
     return t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
 
 
+def _same_strides(a, b, shape):
+    return a == b or all(x == y for x, y, n in zip(a, b, shape) if n != 1)           # (a size-1 dimension's stride is free)
+
+
 def _same_layout(t, p):
-    return t.stride() == p.stride() or all(a == b for a, b, n in zip(t.stride(), p.stride(), p.shape) if n != 1)      # (a size-1 dimension's stride is free)
+    return _same_strides(t.stride(), p.stride(), p.shape)
 
 
-def _like(flat, off, p):
-    """The p.numel() elements of `flat` from `off` on, with p's shape and p's order in memory."""
-    return torch.as_strided(flat, p.size(), p.stride(), flat.storage_offset() + off)
+def _layout(t):
+    return t.size(), t.stride()
+
+
+def _like(flat, off, layout):
+    """The elements of `flat` from `off` on, with the shape and order in memory of _layout(p)."""
+    return torch.as_strided(flat, *layout, flat.storage_offset() + off)
 
 
 class _Table:
@@ -331,7 +339,7 @@ class FusedAdamW(torch.optim.Optimizer):
             table = plan["table"]
             m = torch.empty(plan["total"], dtype=torch.float32, device=self._device())
             v = torch.empty_like(m)
-            torch._foreach_copy_([_like(t, plan["at"][id(p)], p) for t in (m, v) for p, _ in todo], [st[k] for k in ("exp_avg", "exp_avg_sq") for _, st in todo])
+            torch._foreach_copy_([_like(t, plan["at"][id(p)], _layout(p)) for t in (m, v) for p, _ in todo], [st[k] for k in ("exp_avg", "exp_avg_sq") for _, st in todo])
             if table.n_chunks:
                 call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
                      m.data_ptr(), v.data_ptr(), 1, raw_stream())
@@ -370,17 +378,23 @@ class FusedAdamW(torch.optim.Optimizer):
             n = p.numel()
             self.state[p] = {"step": torch.zeros((), dtype=torch.float32), "exp_avg_codes": codes[0, at * _BLOCK:at * _BLOCK + n],
                              "exp_avg_scales": scales[0, at:at + nb], "exp_avg_sq_codes": codes[1, at * _BLOCK:at * _BLOCK + n],
-                             "exp_avg_sq_scales": scales[1, at:at + nb]}
+                             "exp_avg_sq_scales": scales[1, at:at + nb], "layout": _layout(p)}
             at += nb
         at = 0
         for p in wide:
-            self.state[p] = {"step": torch.zeros((), dtype=torch.float32), "exp_avg": _like(moments[0], at, p), "exp_avg_sq": _like(moments[1], at, p)}
+            self.state[p] = {"step": torch.zeros((), dtype=torch.float32), "exp_avg": _like(moments[0], at, _layout(p)), "exp_avg_sq": _like(moments[1], at, _layout(p))}
             at += p.numel()
 
     def _state_tensors(self, ps):
-        return [t for p in ps for k, t in self.state[p].items() if k != "step"]
+        return [t for p in ps for k, t in self.state[p].items() if k not in ("step", "layout")]
+
+    def _state_layout(self, p):
+        """Shape and order in memory that p's state was made for."""
+        st = self.state.get(p)
+        return _layout(p) if not st else st["layout"] if "layout" in st else _layout(st["exp_avg"])
 
     def _records(self, ps, groups):
+        """Rows of a device table, without the gradients' addresses: what the kernels go by is checked here."""
         rows = []
         for p, gi in zip(ps, groups):
             st, n = self.state[p], p.numel()
@@ -395,8 +409,8 @@ class FusedAdamW(torch.optim.Optimizer):
             else:
                 a, b = st["exp_avg"], st["exp_avg_sq"]
                 for t in (a, b):
-                    if t.dtype != torch.float32 or t.shape != p.shape or t.device != p.device or not _same_layout(t, p):
-                        raise BtsAmdError("FusedAdamW: the state of a parameter was replaced by something that is not f32 in the parameter's layout")
+                    if t.dtype != torch.float32 or t.device != p.device or t.numel() != n or not _dense(t) or t.shape != a.shape or not _same_layout(t, a):
+                        raise BtsAmdError("FusedAdamW: the state of a parameter of %d elements was replaced by something else, or is one of %d elements" % (n, t.numel()))
                 rows.append((p.data_ptr(), 0, a.data_ptr(), b.data_ptr(), 0, 0, n, gi, flags))
         return np.array(rows, dtype=_RECORD)
 
@@ -437,6 +451,11 @@ class FusedAdamW(torch.optim.Optimizer):
         if fresh:
             self._new_state(fresh)
             self._state_plan = None
+        for p in ps:
+            shape, strides = self._state_layout(p)
+            if shape != p.shape or not _same_strides(strides, p.stride(), shape):
+                raise BtsAmdError("FusedAdamW: a parameter is %s with strides %s now, its state was made for %s with strides %s -- load_state_dict(state_dict()) "
+                                  "makes it anew" % (tuple(p.shape), p.stride(), tuple(shape), strides))
         rec = self._records(ps, groups)
         rec["g"] = gptr
         self._plan = _Table(rec, [p.numel() for p in ps], self._device())
@@ -462,13 +481,14 @@ class FusedAdamW(torch.optim.Optimizer):
             table = _Table(self._records(hp, [0] * len(hp)), [sizes[i] for i in have], self._device())
             table.holds = (ps, self._state_tensors(hp))
             table.offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
-            self._state_plan = {"key": key, "table": table, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "all": len(have) == len(ps)}
+            self._state_plan = {"key": key, "table": table, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "all": len(have) == len(ps),
+                                "layouts": list(map(self._state_layout, ps))}
         return self._state_plan
 
     @torch.no_grad()
     def moments(self, flat=False):
         """What the states stand for, in f32: a list of (exp_avg, exp_avg_sq) per parameter in the groups' order, shaped like the parameters --
-        or, with flat, two vectors that hold them one after the other (each in its parameter's memory order).  New memory every time;
+        or, with flat, two vectors that hold them one after the other (each in the memory order that its parameter had when its state was made).  New memory every time;
         zeros where a parameter has no state yet.  To be captured into a graph it must have been called once before."""
         if self._elsewhere() is not None:
             with torch.cuda.device(self._elsewhere()):
@@ -486,7 +506,7 @@ class FusedAdamW(torch.optim.Optimizer):
                  m.data_ptr(), v.data_ptr(), 0, stream)
         if flat:
             return m, v
-        return [(_like(m, plan["at"][id(p)], p), _like(v, plan["at"][id(p)], p)) for g in self.param_groups for p in g["params"]]
+        return [(_like(m, at, how), _like(v, at, how)) for at, how in zip(plan["at"].values(), plan["layouts"])]
 
     def _step_multi(self, prepared):
         table = self._step_table()

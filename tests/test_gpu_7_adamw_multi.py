@@ -618,3 +618,28 @@ def test_memory_dropped_while_another_stream_steps():
     feed(qs, 2)
     ob.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and oa.device_steps() == [1.0, 1.0]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_parameter_that_changes_its_order_in_memory(bits):
+    """channels_last between two steps: refused until the state is loaded again, and then right."""
+    torch.manual_seed(71)
+    p = torch.randn(40, 24, 3, 3, device=DEV).requires_grad_(True)
+    opt = optimizer([p], None, state_bits=bits)
+    feed([p], 1)
+    check_step(opt)
+    m, v = (t.clone() for t in opt.moments()[0])
+    p.data = p.data.contiguous(memory_format=torch.channels_last)
+    p.grad = torch.randn_like(p)
+    was = p.detach().clone()
+    with pytest.raises(BtsAmdError):
+        opt.step()
+    assert torch.equal(p, was) and all(torch.equal(a, b) for a, b in zip(opt.moments()[0], (m, v)))
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    m1, v1 = opt.moments()[0]
+    assert m1.stride() == p.stride()
+    if bits == 32:
+        assert torch.equal(m1, m) and torch.equal(v1, v)
+    else:                                                                   # other 256 elements share a scale now
+        assert ((m1 - m).abs() <= 2.0 ** -4 * m.abs() + 2.0 ** -18 * m.abs().max()).all() and ((v1 - v).abs() <= 2.0 ** -4 * v + 2.0 ** -30 * v.max()).all()
+    check_step(opt)

@@ -264,7 +264,7 @@ def test_adamw_memory_outlives_the_work_of_every_stream(stubbed_adamw, monkeypat
     p.grad, q.grad = torch.zeros(9000), torch.zeros(50)
 
     def kept(*more):
-        own = [t for st in opt.state.values() for k, t in st.items() if k != "step"]
+        own = [t for st in opt.state.values() for t in st.values() if torch.is_tensor(t) and t.dim()]
         return {t.untyped_storage().data_ptr() for t in own + list(more) if t is not None}
     opt.step()
     opt.moments()
@@ -288,3 +288,25 @@ def test_adamw_memory_outlives_the_work_of_every_stream(stubbed_adamw, monkeypat
     now[0] = 3
     opt.prepare_step()
     assert (opt._hyper.data_ptr(), 3) in recorded
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_sees_that_a_parameter_changed_its_order_in_memory(stubbed_adamw, bits):
+    """model.to(memory_format=torch.channels_last) between two steps: the codes lie in the old order."""
+    from bts_amd.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(40, 24, 3, 3))
+    opt = FusedAdamW([p], state_bits=bits)
+    p.grad = torch.zeros_like(p)
+    opt.step()
+    opt.moments()
+    p.data = p.data.contiguous(memory_format=torch.channels_last)
+    p.grad = torch.zeros_like(p)
+    n = len(stubbed_adamw)
+    with pytest.raises(_lib.BtsAmdError, match="load_state_dict"):
+        opt.step()
+    assert len(stubbed_adamw) == n
+    assert all(t.shape == p.shape and t.is_contiguous() for t in opt.moments()[0])       # the values where they belong
+    p.data = torch.zeros(40, 24, 3, 3)
+    p.grad = torch.zeros_like(p)
+    opt.step()
+    assert stubbed_adamw[-1][0] == "bts_adamw_multi_step"
