@@ -528,7 +528,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 self._norm.zero_()
             return
         if torch.cuda.is_current_stream_capturing():
-            self._kept.append((table.records, table.chunks, rows, table.holds, [p.grad for p in table.holds[0]]))
+            # the memory itself: a parameter or gradient that is given other memory (p.data = ...) does not take this from the graph
+            self._kept.append((table.records, table.chunks, rows, table.holds, [t.detach() for p in table.holds[0] for t in (p, p.grad)]))
         if profiler.ACTIVE is not None:
             profiler.note("adamw_multi_step", "hbm", float(self._bytes))
         call("bts_adamw_multi_step", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, rows.data_ptr(), len(self.param_groups), hyper,

@@ -643,3 +643,23 @@ def test_a_parameter_that_changes_its_order_in_memory(bits):
     else:                                                                   # other 256 elements share a scale now
         assert ((m1 - m).abs() <= 2.0 ** -4 * m.abs() + 2.0 ** -18 * m.abs().max()).all() and ((v1 - v).abs() <= 2.0 ** -4 * v + 2.0 ** -30 * v.max()).all()
     check_step(opt)
+
+
+def test_a_graph_outlives_the_memory_of_its_parameters():
+    """Parameter and gradient are given other memory after the capture: a replay writes what it was captured with, and nothing else."""
+    ps = tensors([9000, 333], torch.float32, 73)
+    opt = optimizer(ps, 1, state_bits=8, max_grad_norm=0.5)
+    feed(ps, 1)
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step(prepared=True)
+    for p in ps:
+        p.data = p.data.clone()
+        p.grad = None
+    torch.cuda.synchronize()
+    now = [p.detach().clone() for p in ps]
+    fence = [torch.full((n,), 3.0, device=DEV) for n in (9000, 333) * 64]   # takes what the allocator has free
+    g.replay()
+    torch.cuda.synchronize()
+    assert all((t == 3.0).all() for t in fence) and all(torch.equal(p, n) for p, n in zip(ps, now))

@@ -310,3 +310,23 @@ def test_adamw_sees_that_a_parameter_changed_its_order_in_memory(stubbed_adamw, 
     p.grad = torch.zeros_like(p)
     opt.step()
     assert stubbed_adamw[-1][0] == "bts_adamw_multi_step"
+
+
+def test_adamw_captured_steps_keep_the_memory_of_parameters_and_gradients(stubbed_adamw, monkeypatch):
+    """A graph goes on writing the addresses that it was captured with, also after p.data was given other memory."""
+    from bts_amd.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(5000))
+    opt = FusedAdamW([p], state_bits=8)
+    p.grad = torch.zeros(5000)
+    opt.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    opt.step(prepared=True)
+    rec = stubbed_adamw[-1][1]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    p.data, p.grad.data = torch.zeros(5000), torch.zeros(5000)
+    p.grad = None
+
+    def tensors(x):
+        return [x] if torch.is_tensor(x) else [t for y in x for t in tensors(y)] if isinstance(x, (list, tuple)) else []
+    kept = {t.data_ptr() for t in tensors(opt._kept)}
+    assert {int(rec["p"][0]), int(rec["g"][0]), int(rec["m"][0]), int(rec["v"][0])} <= kept
