@@ -4,14 +4,18 @@ The decoder normalises with BatchNorm (bts.py:155-172), whose statistics are tak
 not depend on the batch.  ``LayerNorm`` takes the place of ``torch.nn.LayerNorm`` (same arguments, parameters and state-dict keys),
 ``LayerNorm2d`` normalises the channels at every pixel of an NCHW map, where ``nn.BatchNorm2d`` would normalise the batch.
 
-Inputs are f32 or bf16, parameters and their gradients f32, statistics f32.  No second derivatives, no CPU path.
+Inputs are f32 or bf16, parameters and their gradients f32, statistics f32.  No second and no forward-mode derivatives, no
+torch.jit.trace (all refused), no CPU path.
 """
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
 from ._lib import BtsAmdError
+
+_is_tracing = torch._C._is_tracing
 
 __all__ = ["layer_norm", "LayerNorm", "LayerNorm2d"]
 
@@ -61,7 +65,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., C], 1 <= C <= 16384; weight and bias f32 [C] or None."""
     if x.dim() == 0:
         raise BtsAmdError("layer_norm: x must have at least one axis")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if _is_tracing():
+        raise BtsAmdError("layer_norm cannot be traced: torch.jit.trace would record the allocation of its result and no launch")
+    # forward-mode differentiation sees the call only through the Function, which refuses a tangent (a dual tensor does not require gradients)
+    if (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
+            or forward_ad._current_level >= 0):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return ops.layer_norm_fwd_rows(*_rows(x), weight, bias, float(eps), False)
 

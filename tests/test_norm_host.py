@@ -330,3 +330,28 @@ def test_adamw_captured_steps_keep_the_memory_of_parameters_and_gradients(stubbe
         return [x] if torch.is_tensor(x) else [t for y in x for t in tensors(y)] if isinstance(x, (list, tuple)) else []
     kept = {t.data_ptr() for t in tensors(opt._kept)}
     assert {int(rec["p"][0]), int(rec["g"][0]), int(rec["m"][0]), int(rec["v"][0])} <= kept
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_derivatives_are_refused(stubbed_norm, needs_grad):
+    import torch.autograd.forward_ad as forward_ad
+    x, w, b = torch.randn(3, 8), torch.ones(8), torch.zeros(8)
+    w.requires_grad_(needs_grad)
+    with forward_ad.dual_level():
+        assert layer_norm(x, w, b).shape == x.shape                       # no tangent anywhere: nothing is lost
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for i in range(3):
+                    args = [x, w.detach(), b]
+                    args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                    with pytest.raises(NotImplementedError):
+                        layer_norm(*args)
+    n = len(stubbed_norm)
+    assert layer_norm(x, w.detach(), b).shape == x.shape and len(stubbed_norm) == n + 1
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_tracing_is_refused(stubbed_norm, needs_grad):
+    with pytest.raises(_lib.BtsAmdError, match="traced"):
+        torch.jit.trace(LayerNorm(8).requires_grad_(needs_grad), torch.randn(3, 8), check_trace=False)
+    assert not stubbed_norm and LayerNorm(8)(torch.randn(3, 8)).shape == (3, 8)
