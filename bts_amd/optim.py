@@ -200,6 +200,10 @@ class FusedAdamW(torch.optim.Optimizer):
             st = self.state.get(p)
             if st and "step" in st:
                 seen.add(float(st["step"]))
+        return self._one_step(seen)
+
+    @staticmethod
+    def _one_step(seen):
         if len(seen) > 1:
             raise BtsAmdError("FusedAdamW keeps one step count per parameter group; this state has steps %s inside one group "
                               "(load it with torch.optim.AdamW, or regroup the parameters)" % sorted(seen))
@@ -300,7 +304,11 @@ class FusedAdamW(torch.optim.Optimizer):
         return sd
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+        check = self.register_load_state_dict_pre_hook(lambda _, sd: self._check_loaded(sd))       # behind all others, before anything changes
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            check.remove()
         # the moment buffers were replaced and the step count comes from the checkpoint: drop every cached pointer
         # table and rebuild the device rows (step, betas, lr) from what was just loaded
         self._tables = {}
@@ -314,23 +322,30 @@ class FusedAdamW(torch.optim.Optimizer):
                         st[k] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(st[k])
         self._rows()
 
+    def _check_loaded(self, state_dict):
+        """Refuses a checkpoint that does not fit while this optimizer is still whole."""
+        saved = state_dict["param_groups"]
+        if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
+            return                                  # (refused by what comes next)
+        todo = []
+        for g, sg in zip(self.param_groups, saved):
+            there = [(i, p, state_dict["state"][i]) for i, p in zip(sg["params"], g["params"]) if state_dict["state"].get(i)]
+            self._one_step({float(st["step"]) for _, _, st in there if "step" in st})
+            todo += there
+        if self._multi and todo:
+            for i, p, st in todo:
+                if "step" not in st or any(k not in st or tuple(st[k].shape) != tuple(p.shape) for k in ("exp_avg", "exp_avg_sq")):
+                    raise BtsAmdError("FusedAdamW.load_state_dict: parameter %r needs step, and exp_avg and exp_avg_sq of shape %s" % (i, tuple(p.shape)))
+            self._check_parameters([p for _, p, _ in todo])
+
     # ---- 8-bit / multi-tensor form -------------------------------------------------------------------
     def _load_moments(self, state_dict):
         ps = [p for g in self.param_groups for p in g["params"]]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         self.state.clear()
-        todo = []
-        for i, p in zip(ids, ps):
-            st = state_dict["state"].get(i)
-            if not st:
-                continue
-            for k in ("exp_avg", "exp_avg_sq"):
-                if k not in st or tuple(st[k].shape) != tuple(p.shape):
-                    raise BtsAmdError("FusedAdamW.load_state_dict: parameter %r needs %s of shape %s" % (i, k, tuple(p.shape)))
-            todo.append((p, st))
+        todo = [(p, state_dict["state"][i]) for i, p in zip(ids, ps) if state_dict["state"].get(i)]
         if not todo:
             return
-        self._check_parameters([p for p, _ in todo])
         self._new_state([p for p, _ in todo])
         for p, st in todo:
             self.state[p]["step"] = torch.as_tensor(st["step"], dtype=torch.float32).reshape(()).cpu().clone()

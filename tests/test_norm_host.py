@@ -355,3 +355,38 @@ def test_tracing_is_refused(stubbed_norm, needs_grad):
     with pytest.raises(_lib.BtsAmdError, match="traced"):
         torch.jit.trace(LayerNorm(8).requires_grad_(needs_grad), torch.randn(3, 8), check_trace=False)
     assert not stubbed_norm and LayerNorm(8)(torch.randn(3, 8)).shape == (3, 8)
+
+
+@pytest.mark.parametrize("kw", [dict(state_bits=8), dict(state_bits=32), dict()])
+def test_adamw_a_refused_checkpoint_changes_nothing(stubbed_adamw, kw):
+    import copy
+    from bts_amd.optim import FusedAdamW
+    p, q = torch.nn.Parameter(torch.zeros(5000)), torch.nn.Parameter(torch.zeros(50))
+    opt = FusedAdamW([{"params": [p, q], "lr": 0.5}], **kw)
+    if kw:
+        p.grad, q.grad = torch.zeros(5000), torch.zeros(50)
+        opt.step()
+        good = opt.state_dict()
+    else:                                                       # (its step has no form without a GPU)
+        good = {"state": {i: {"step": torch.tensor(1.0), "exp_avg": torch.zeros(n), "exp_avg_sq": torch.zeros(n)} for i, n in ((0, 5000), (1, 50))},
+                "param_groups": opt.state_dict()["param_groups"]}
+        opt.load_state_dict(good)
+    had = {id(t): {k: v for k, v in st.items()} for t, st in opt.state.items()}
+    hyper = opt._hyper
+    bads = [lambda sd: sd["state"][1].update(step=torch.tensor(7.0))]
+    if kw:
+        bads += [lambda sd: sd["state"][1].update(exp_avg=torch.zeros(3)), lambda sd: sd["state"][0].pop("exp_avg_sq"), lambda sd: sd["state"][1].pop("step")]
+    for bad in bads:
+        sd = copy.deepcopy(good)
+        sd["param_groups"][0]["lr"] = 0.25
+        bad(sd)
+        with pytest.raises(_lib.BtsAmdError):
+            opt.load_state_dict(sd)
+        assert opt.param_groups[0]["lr"] == 0.5 and opt._hyper is hyper
+        assert {id(t): set(st) for t, st in opt.state.items()} == {t: set(st) for t, st in had.items()}
+        assert all(st[k] is had[id(t)][k] for t, st in opt.state.items() for k in st if k != "step")
+    with pytest.raises(ValueError):                             # torch's own refusal
+        opt.load_state_dict({"state": {}, "param_groups": []})
+    if kw:
+        opt.step()
+        assert stubbed_adamw[-1][0] == "bts_adamw_multi_step"
