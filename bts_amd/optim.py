@@ -294,21 +294,34 @@ class FusedAdamW(torch.optim.Optimizer):
         """torch.optim.AdamW layout; the per-parameter ``step`` entries are refreshed from the device counter first
         (they are not touched by step(), which may be running inside a replayed graph)."""
         self._refresh_steps()
-        sd = super().state_dict()
-        if self._multi and self.state:
-            ps = [p for g in self.param_groups for p in g["params"]]
-            for i, (p, (m, v)) in enumerate(zip(ps, self.moments())):
-                st = self.state.get(p)
-                if st:
-                    sd["state"][i] = {"step": st["step"], "exp_avg": m, "exp_avg_sq": v}
-        return sd
+        if not (self._multi and self.state):
+            return super().state_dict()
+        put = self.register_state_dict_post_hook(FusedAdamW._put_moments, prepend=True)                 # before the user's hooks
+        try:
+            return super().state_dict()
+        finally:
+            put.remove()
+
+    def _put_moments(self, sd):
+        ps = [p for g in self.param_groups for p in g["params"]]
+        for i, (p, (m, v)) in enumerate(zip(ps, self.moments())):
+            st = self.state.get(p)
+            if st:
+                sd["state"][i] = {"step": st["step"], "exp_avg": m, "exp_avg_sq": v}
 
     def load_state_dict(self, state_dict):
-        check = self.register_load_state_dict_pre_hook(lambda _, sd: self._check_loaded(sd))       # behind all others, before anything changes
+        # Between the user's hooks: what their pre hooks made of the checkpoint counts, and is checked before anything changes; their post
+        # hooks find the optimizer whole.
+        last = []
+        check = self.register_load_state_dict_pre_hook(lambda _, sd: last.append(self._check_loaded(sd)))
+        rebuild = self.register_load_state_dict_post_hook(lambda _: self._loaded(last[-1]), prepend=True)
         try:
             super().load_state_dict(state_dict)
         finally:
             check.remove()
+            rebuild.remove()
+
+    def _loaded(self, state_dict):
         # the moment buffers were replaced and the step count comes from the checkpoint: drop every cached pointer
         # table and rebuild the device rows (step, betas, lr) from what was just loaded
         self._tables = {}
@@ -326,7 +339,7 @@ class FusedAdamW(torch.optim.Optimizer):
         """Refuses a checkpoint that does not fit while this optimizer is still whole."""
         saved = state_dict["param_groups"]
         if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
-            return                                  # (refused by what comes next)
+            return state_dict                       # (refused by what comes next)
         todo = []
         for g, sg in zip(self.param_groups, saved):
             there = [(i, p, state_dict["state"][i]) for i, p in zip(sg["params"], g["params"]) if state_dict["state"].get(i)]
@@ -337,6 +350,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 if "step" not in st or any(k not in st or tuple(st[k].shape) != tuple(p.shape) for k in ("exp_avg", "exp_avg_sq")):
                     raise BtsAmdError("FusedAdamW.load_state_dict: parameter %r needs step, and exp_avg and exp_avg_sq of shape %s" % (i, tuple(p.shape)))
             self._check_parameters([p for _, p, _ in todo])
+        return state_dict
 
     # ---- 8-bit / multi-tensor form -------------------------------------------------------------------
     def _load_moments(self, state_dict):

@@ -663,3 +663,42 @@ def test_a_graph_outlives_the_memory_of_its_parameters():
     g.replay()
     torch.cuda.synchronize()
     assert all((t == 3.0).all() for t in fence) and all(torch.equal(p, n) for p, n in zip(ps, now))
+
+
+@pytest.mark.parametrize("kw", [dict(state_bits=8), dict(max_grad_norm=1.0), dict()])
+def test_state_dict_hooks_see_and_change_the_moments(kw):
+    """torch's contract: a post hook of state_dict sees what is returned, what a pre hook of load_state_dict returns is loaded, and its post
+    hook finds the state in place."""
+    ps = tensors([5000, 40], torch.float32, 79)
+    opt = optimizer(ps, 1, **kw)
+    feed(ps, 1)
+    opt.step()
+    seen = []
+
+    def after(o, sd):
+        seen.append({i: st["exp_avg"].clone() for i, st in sd["state"].items()})
+        for i, st in sd["state"].items():                                   # (without options these dicts are the optimizer's own: not in place)
+            sd["state"][i] = {**st, "exp_avg": st["exp_avg"] * 2.0}
+    handles = [opt.register_state_dict_post_hook(after)]
+    sd = opt.state_dict()
+    handles[0].remove()
+    plain_sd = copy.deepcopy(opt.state_dict())
+    for i in (0, 1):
+        assert torch.equal(seen[0][i], plain_sd["state"][i]["exp_avg"]) and torch.equal(sd["state"][i]["exp_avg"], 2.0 * seen[0][i])
+
+    def before(o, sd):
+        sd = copy.deepcopy(sd)
+        for st in sd["state"].values():
+            st["exp_avg"] = st["exp_avg"] * 4.0
+            st["step"] = torch.tensor(9.0)
+        return sd
+    found = []
+    handles = [opt.register_load_state_dict_pre_hook(before), opt.register_load_state_dict_post_hook(lambda o: found.append((o.state_dict(), o.device_steps())))]
+    opt.load_state_dict(plain_sd)
+    for h in handles:
+        h.remove()
+    now = opt.state_dict()
+    assert opt.device_steps() == found[0][1] == [9.0, 9.0] and plain_sd["state"][0]["step"] == 1.0
+    for i in (0, 1):                                                        # times a power of two: exact in 8 bits
+        assert torch.equal(now["state"][i]["exp_avg"], 4.0 * plain_sd["state"][i]["exp_avg"]) and torch.equal(found[0][0]["state"][i]["exp_avg"], now["state"][i]["exp_avg"])
+    assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks and not opt._optimizer_state_dict_post_hooks
