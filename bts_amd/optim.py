@@ -34,9 +34,10 @@ Options beyond that, all on `bts_adamw_multi_step` (csrc/adamw.hip; one update l
   ``grad_norm`` is a device tensor that every step rewrites.  ``float('inf')`` only measures.
 * bf16 parameters (with bf16 gradients; states stay f32 or 8-bit, the update is formed in f32 and rounded once).
 
-There, states are replaced through ``load_state_dict`` only, and the learning rate is a launch argument: a captured step takes
-``prepared=True`` and ``prepare_step()`` outside the graph, as above.  A captured step works on the gradients, states and step counts that it was
-captured with: capture again after ``load_state_dict`` or ``add_param_group``.
+There, the tensors of a state are replaced through ``load_state_dict`` only (a state may be reset: ``opt.state = defaultdict(dict)``,
+``opt.state[p] = {}``), and the learning rate is a launch argument: a captured step takes ``prepared=True`` and ``prepare_step()`` outside the
+graph, as above.  A captured step works on the parameters' memory, gradients, states and step counts that it was captured with, and the
+optimizer keeps them: capture again after ``load_state_dict`` or ``add_param_group``.
 """
 import ctypes as C
 import itertools
@@ -104,6 +105,7 @@ class _Table:
         chunks[:, 1] = np.arange(self.n_chunks) - np.repeat(np.cumsum(counts) - counts, counts)
         self.host = records
         self.holds = self.offsets = None        # what must live as long as the addresses; begin of each tensor in flat moments
+        self.states = None                      # _states_now() when it was made
         self.chunks = torch.from_numpy(chunks).to(device)
         self.records = torch.from_numpy(records.view(np.uint8)).to(device)
         self.records_on, self.used_on = raw_stream(), set()
@@ -422,6 +424,14 @@ class FusedAdamW(torch.optim.Optimizer):
         st = self.state.get(p)
         return _layout(p) if not st else st["layout"] if "layout" in st else _layout(st["exp_avg"])
 
+    def _states_now(self):
+        return self.state, list(self.state.values()), list(map(len, self.state.values()))
+
+    def _same_states(self, then):
+        """The states are the dicts that they were, and none was emptied."""
+        state, dicts, lens = then
+        return self.state is state and len(state) == len(dicts) and all(map(is_, state.values(), dicts)) and list(map(len, dicts)) == lens
+
     def _records(self, ps, groups):
         """Rows of a device table, without the gradients' addresses: what the kernels go by is checked here."""
         rows = []
@@ -458,7 +468,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if not ps:
             return None
         seen = (lens, keep, list(map(_ptr, ps)), list(map(_numel, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
-        if self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])):
+        if self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])) and self._same_states(self._plan.states):
             if gptr == self._gptr:
                 return self._plan
             if list(map(_numel, gs)) == seen[3]:
@@ -488,7 +498,7 @@ class FusedAdamW(torch.optim.Optimizer):
         rec = self._records(ps, groups)
         rec["g"] = gptr
         self._plan = _Table(rec, [p.numel() for p in ps], self._device())
-        self._plan.holds = (ps, self._state_tensors(ps))        # the addresses in the table stay theirs
+        self._plan.holds, self._plan.states = (ps, self._state_tensors(ps)), self._states_now()     # the addresses in the table stay theirs
         self._seen, self._gptr = seen, gptr
         self._bytes = sum(p.numel() * (3 * p.element_size() + (4 if self._is_8bit(p) else 16)) for p in ps)
         return self._plan
@@ -501,14 +511,14 @@ class FusedAdamW(torch.optim.Optimizer):
         """The table of all parameters that have a state, for bts_adamw_multi_moments, and where each begins in flat moments."""
         ps = [p for g in self.param_groups for p in g["params"]]
         sizes = list(map(_numel, ps))
-        key = (list(map(id, ps)), sizes, len(self.state))
-        if self._state_plan is None or self._state_plan["key"] != key:
+        key = (list(map(id, ps)), sizes)
+        if self._state_plan is None or self._state_plan["key"] != key or not self._same_states(self._state_plan["table"].states):
             self._no_capture("moments", "call moments() once")
             offs = [0] + list(itertools.accumulate(sizes))
             have = [i for i, p in enumerate(ps) if self.state.get(p)]
             hp = [ps[i] for i in have]
             table = _Table(self._records(hp, [0] * len(hp)), [sizes[i] for i in have], self._device())
-            table.holds = (ps, self._state_tensors(hp))
+            table.holds, table.states = (ps, self._state_tensors(hp)), self._states_now()
             table.offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
             self._state_plan = {"key": key, "table": table, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "all": len(have) == len(ps),
                                 "layouts": list(map(self._state_layout, ps))}

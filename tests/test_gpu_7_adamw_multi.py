@@ -702,3 +702,16 @@ def test_state_dict_hooks_see_and_change_the_moments(kw):
     for i in (0, 1):                                                        # times a power of two: exact in 8 bits
         assert torch.equal(now["state"][i]["exp_avg"], 4.0 * plain_sd["state"][i]["exp_avg"]) and torch.equal(found[0][0]["state"][i]["exp_avg"], now["state"][i]["exp_avg"])
     assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks and not opt._optimizer_state_dict_post_hooks
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_that_were_reset_begin_at_zero(bits):
+    from collections import defaultdict
+    ps = tensors([5000, 333], torch.float32, 83)
+    opt = optimizer(ps, 1, state_bits=bits)
+    for reset in (lambda: None, lambda: setattr(opt, "state", defaultdict(dict)), lambda: opt.state.update({ps[0]: {}}), lambda: opt.state.clear()):
+        feed(ps, 1)
+        check_step(opt)
+        reset()
+    assert all((t == 0).all() for mv in opt.moments() for t in mv)
+    check_step(opt)

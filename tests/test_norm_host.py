@@ -390,3 +390,38 @@ def test_adamw_a_refused_checkpoint_changes_nothing(stubbed_adamw, kw):
     if kw:
         opt.step()
         assert stubbed_adamw[-1][0] == "bts_adamw_multi_step"
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_sees_that_states_were_reset(stubbed_adamw, bits):
+    from collections import defaultdict
+    from bts_amd.optim import FusedAdamW
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in (5000, 50, 6000)]
+    opt = FusedAdamW(ps, state_bits=bits)
+    for p in ps:
+        p.grad = torch.zeros_like(p)
+
+    def step():
+        opt.step()
+        rec = stubbed_adamw[-1][1]
+        opt.moments()
+        seen = stubbed_adamw[-1][1]
+        own = [opt.state[p]["exp_avg_codes" if "exp_avg_codes" in opt.state[p] else "exp_avg"].data_ptr() for p in ps]
+        assert rec["m"].tolist() == seen["m"].tolist() == own and set(opt.state_dict()["state"]) == {0, 1, 2}
+        return [opt.state[p] for p in ps]
+    first = step()
+    assert all(a is b for a, b in zip(first, step()))
+    opt.state = defaultdict(dict)
+    second = step()
+    assert not any(a is b for a, b in zip(first, second))
+    opt.state[ps[1]] = {}
+    third = step()
+    assert [a is b for a, b in zip(second, third)] == [True, False, True]
+    opt.state.pop(ps[2])
+    fourth = step()
+    opt.state[ps[0]].clear()
+    step()
+    opt.state.clear()
+    assert not any(a is b for a, b in zip(fourth, step()))
+    opt.state.clear()
+    assert all((t == 0).all() for mv in opt.moments() for t in mv) and not opt.state_dict()["state"]
