@@ -448,8 +448,10 @@ __global__ __launch_bounds__(1024) void adamw_begin_kernel(double* __restrict__ 
             for (int i = 0; i < 16; ++i) t += red[i];
             t = sqrt(t);
             *grad_norm = (float)t;
-            c = (set ? hh.max_norm : tail[0]) / (t + 1e-6);
+            const double most = set ? hh.max_norm : tail[0];
+            c = most / (t + 1e-6);
             c = c > 1.0 ? 1.0 : c;                                  // a norm that is NaN makes c NaN, and with it every parameter
+            if (most == __builtin_inf()) c = 1.0;                   // only measured: whatever the norm is
         }
         if (advance) tail[1] = c;
     }

@@ -31,7 +31,8 @@ Options beyond that, all on `bts_adamw_multi_step` (csrc/adamw.hip; one update l
   state -- from here, or from the reference's optimizer -- forms the codes again: values that came from codes give the same values.
 * ``max_grad_norm``: the gradients of all groups are scaled by min(1, max_grad_norm / (norm + 1e-6)) inside the step, where norm is their
   common 2-norm (torch.nn.utils.clip_grad_norm_'s rule; the gradients themselves stay as they are).  No host synchronisation:
-  ``grad_norm`` is a device tensor that every step rewrites.  ``float('inf')`` only measures.
+  ``grad_norm`` is a device tensor that every step rewrites.  ``float('inf')`` only measures: gradients that are not finite stay
+  their own elements' matter, where a finite bound makes every parameter NaN for a norm that is (clip_grad_norm_'s rule).
 * bf16 parameters (with bf16 gradients; states stay f32 or 8-bit, the update is formed in f32 and rounded once).
 
 There, the tensors of a state are replaced through ``load_state_dict`` only (a state may be reset: ``opt.state = defaultdict(dict)``,

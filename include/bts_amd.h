@@ -520,7 +520,7 @@ int bts_layernorm_bwd(const void* dy, long dy_stride, const void* x, long x_stri
 
 /* ------------------------------------------------------------------------------------
  * AdamW over many tensors with states in 32 or in 8 bits, f32 or bf16 parameters, optionally clipped by the global gradient norm:
- *     c = min(1, max_norm / (|g| + 1e-6)) over ALL gradients of the call (1 without clipping), g' = c g
+ *     c = min(1, max_norm / (|g| + 1e-6)) over ALL gradients of the call (1 without clipping and for max_norm = infinity), g' = c g
  *     m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g' g'   (8-bit states: each product and sum rounded to 64 bits, in this order)
  *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * tensors [n] and chunks [n_chunks][2] = {tensor, i: its elements from BTS_ADAMW_CHUNK i on} are on the DEVICE; every chunk of

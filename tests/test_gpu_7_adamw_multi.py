@@ -715,3 +715,20 @@ def test_states_that_were_reset_begin_at_zero(bits):
         reset()
     assert all((t == 0).all() for mv in opt.moments() for t in mv)
     check_step(opt)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_infinite_bound_only_measures(bits):
+    """Also where the norm is infinite or NaN: the step is the one without a bound."""
+    for bad in (float("inf"), float("nan"), -float("inf")):
+        ps, qs = tensors([5000, 333], torch.float32, 89), tensors([5000, 333], torch.float32, 89)
+        oa, ob = optimizer(ps, 1, state_bits=bits, max_grad_norm=float("inf")), optimizer(qs, 1, state_bits=bits)
+        feed(ps, 1)
+        feed(qs, 1)
+        ps[0].grad[17] = qs[0].grad[17] = bad
+        oa.step()
+        ob.step()
+        assert not torch.isfinite(oa.grad_norm) and torch.isnan(oa.grad_norm) == (bad != bad)
+        for p, q in zip(ps, qs):
+            assert torch.equal(torch.nan_to_num(p), torch.nan_to_num(q)) and torch.isnan(p).sum() == torch.isnan(q).sum() <= 1
+        assert torch.isfinite(ps[1]).all()
