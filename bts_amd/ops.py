@@ -492,8 +492,8 @@ def _ln_rows(t, what, like=None):
 
 def _ln_vec(t, n, dev, what):
     """Address of an f32 vector of n elements on device dev."""
-    if t.dtype != torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
-        raise BtsAmdError("%s must be a contiguous f32 tensor of %d elements on device %d, got %s %s on %s" % (what, n, dev, tuple(t.shape), t.dtype, t.device))
+    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise BtsAmdError("%s must be a contiguous f32 vector of %d elements on device %d, got %s %s on %s" % (what, n, dev, tuple(t.shape), t.dtype, t.device))
     return t.data_ptr()
 
 
@@ -541,9 +541,9 @@ def layer_norm_bwd(dy, x, stats, weight=None, want_dx=True, want_dweight=True, w
             return layer_norm_bwd(dy, x, stats, weight, want_dx, want_dweight, want_dbias)
     rows = _ln_rows(x, "layer_norm_bwd")
     _, dys = _ln_rows(dy, "layer_norm_bwd: dy", x)
-    if stats is None:
-        raise BtsAmdError("layer_norm_bwd needs the stats of layer_norm_fwd(..., want_stats=True)")
-    _ln_vec(stats, 2 * rows[0], dev, "layer_norm_bwd: stats")
+    if stats is None or not stats.is_contiguous():
+        raise BtsAmdError("layer_norm_bwd needs the stats of layer_norm_fwd(..., want_stats=True), contiguous")
+    _ln_vec(stats.view(-1), 2 * rows[0], dev, "layer_norm_bwd: stats")
     if weight is not None:
         _ln_vec(weight, x.shape[-1], dev, "layer_norm_bwd: weight")
     return layer_norm_bwd_unchecked(dy, dys, x, rows, stats, weight, want_dx, want_dweight, want_dbias)

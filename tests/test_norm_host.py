@@ -425,3 +425,21 @@ def test_adamw_sees_that_states_were_reset(stubbed_adamw, bits):
     assert not any(a is b for a, b in zip(fourth, step()))
     opt.state.clear()
     assert all((t == 0).all() for mv in opt.moments() for t in mv) and not opt.state_dict()["state"]
+
+
+def test_parameters_of_another_shape_are_refused_before_the_launch(monkeypatch):
+    """[1, C] has C elements, but its gradient would come back as [C]."""
+    monkeypatch.setattr(_lib, "require_gpu", lambda t: None)
+    monkeypatch.setattr(ops, "current_device", lambda: -1)
+    monkeypatch.setattr(ops, "raw_stream", lambda: 0)
+    launches = []
+    monkeypatch.setattr(ops, "call", lambda *a: launches.append(a[0]))
+    x = torch.randn(3, 8)
+    for shape in ((1, 8), (8, 1), (2, 4), (7,), ()):
+        for args in ((torch.ones(shape), torch.zeros(8)), (torch.ones(8), torch.zeros(shape)), (torch.ones(shape).requires_grad_(True), None)):
+            with pytest.raises(_lib.BtsAmdError, match="vector"):
+                layer_norm(x, *args)
+    assert not launches
+    layer_norm(x, torch.ones(8), torch.zeros(8))
+    LayerNorm((2, 4))(x.view(3, 2, 4))
+    assert launches == ["bts_layernorm_fwd"] * 2
