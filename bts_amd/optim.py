@@ -158,23 +158,26 @@ class FusedAdamW(torch.optim.Optimizer):
         self._tables = {}
         self._hyper = None          # [n_groups, 8] f32 on the device (bts_adamw_step), or [n_groups + 1, 16] f64 (bts_adamw_multi_step)
         self._seen = self._plan = self._state_plan = None
+        self._steps = None          # step counts of the groups while there are no device rows, where the states do not say them
         self._kept = []             # what captured graphs refer to
         self._scratch = self._norm = None
         self._used_on = set()       # streams that _hyper, _scratch and _norm are recorded for
 
     def __getstate__(self):         # copies and pickles: states with their step counts, nothing that holds addresses
         self._refresh_steps()
-        return {**super().__getstate__(), "_options": self._options, "_multi": self._multi}
+        return {**super().__getstate__(), "_options": self._options, "_multi": self._multi, "_steps": self.device_steps()}
 
     def __setstate__(self, state):  # (load_state_dict calls it too, with the loaded states and groups)
         super().__setstate__(state)
         if "_options" in state:
             self._forget()
+            self._steps = state.get("_steps")
 
     def add_param_group(self, param_group):
         old = getattr(self, "_hyper", None)
         if old is not None:         # the device rows have one row per group: keep their step counts, make them anew
             self._refresh_steps()
+            self._steps = self.device_steps()
             self._hyper = None
         super().add_param_group(param_group)
         self._seen = None
@@ -212,21 +215,28 @@ class FusedAdamW(torch.optim.Optimizer):
                               "(load it with torch.optim.AdamW, or regroup the parameters)" % sorted(seen))
         return seen.pop() if seen else 0.0
 
+    def _group_steps(self):
+        """Step counts without device rows: carried over from earlier ones (a group that took steps without gradients has no state to say
+        it), else what the states say."""
+        known = self._steps or []
+        return [known[gi] if gi < len(known) else self._group_step_from_state(g) for gi, g in enumerate(self.param_groups)]
+
     def _rows(self):
         """The device rows, created on first use from the groups' hyper-parameters and recorded state."""
         if self._hyper is None:
             self._used_on = set()
+            steps, self._steps = self._group_steps(), None
             if self._multi:
                 rows = np.zeros((len(self.param_groups) + 1, _WIDE_ROW))
-                for r, g in zip(rows, self.param_groups):
-                    r[0], r[3], r[4:6], r[6], r[7] = float(g["lr"]), self._group_step_from_state(g), g["betas"], g["eps"], g["weight_decay"]
+                for r, g, t in zip(rows, self.param_groups, steps):
+                    r[0], r[3], r[4:6], r[6], r[7] = float(g["lr"]), t, g["betas"], g["eps"], g["weight_decay"]
                 rows[-1, 0] = math.inf if self.max_grad_norm is None else self.max_grad_norm
                 self._hyper = torch.from_numpy(rows).to(self._device())
                 return self._hyper
             rows = []
-            for g in self.param_groups:
+            for g, t in zip(self.param_groups, steps):
                 b1, b2 = g["betas"]
-                rows.append([float(g["lr"]), 1.0, 1.0, self._group_step_from_state(g), float(b1), float(b2), 0.0, 0.0])
+                rows.append([float(g["lr"]), 1.0, 1.0, t, float(b1), float(b2), 0.0, 0.0])
             self._hyper = torch.tensor(rows, dtype=torch.float32).to(self._device())
         return self._hyper
 
@@ -265,7 +275,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def device_steps(self):
         """Per-group step counts as python floats (synchronises)."""
         if self._hyper is None:
-            return [self._group_step_from_state(g) for g in self.param_groups]
+            return self._group_steps()
         return [float(v) for v in self._hyper[:len(self.param_groups), 3].cpu()]
 
     def _refresh_steps(self):
@@ -328,7 +338,7 @@ class FusedAdamW(torch.optim.Optimizer):
         # the moment buffers were replaced and the step count comes from the checkpoint: drop every cached pointer
         # table and rebuild the device rows (step, betas, lr) from what was just loaded
         self._tables = {}
-        self._hyper = self._seen = self._plan = self._state_plan = None
+        self._hyper = self._seen = self._plan = self._state_plan = self._steps = None
         if self._multi:
             self._load_moments(state_dict)
         else:

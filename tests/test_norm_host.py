@@ -443,3 +443,24 @@ def test_parameters_of_another_shape_are_refused_before_the_launch(monkeypatch):
     layer_norm(x, torch.ones(8), torch.zeros(8))
     LayerNorm((2, 4))(x.view(3, 2, 4))
     assert launches == ["bts_layernorm_fwd"] * 2
+
+
+def test_adamw_steps_without_gradients_are_not_forgotten(stubbed_adamw, monkeypatch):
+    import contextlib
+    import copy
+    from bts_amd import optim
+    p = torch.nn.Parameter(torch.zeros(50))
+    opt = optim.FusedAdamW([p], state_bits=8)
+    opt.step()                                                  # no gradient: no state, but the count goes on
+    opt.step()
+    assert opt.device_steps() == [2.0] and copy.deepcopy(opt).device_steps() == [2.0]
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
+    assert opt.device_steps() == [2.0, 0.0, 0.0]
+    opt.step()
+    assert opt.device_steps() == [3.0, 1.0, 1.0] and copy.deepcopy(opt).device_steps() == [3.0, 1.0, 1.0]
+    sd = opt.state_dict()
+    sd["state"] = {0: {"step": torch.tensor(8.0), "exp_avg": torch.zeros(50), "exp_avg_sq": torch.zeros(50)}}
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    opt.load_state_dict(sd)                                     # what a checkpoint says counts
+    assert opt.device_steps() == [8.0, 0.0, 0.0]
