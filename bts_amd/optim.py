@@ -511,7 +511,8 @@ class FusedAdamW(torch.optim.Optimizer):
         self._plan = _Table(rec, [p.numel() for p in ps], self._device())
         self._plan.holds, self._plan.states = (ps, self._state_tensors(ps)), self._states_now()     # the addresses in the table stay theirs
         self._seen, self._gptr = seen, gptr
-        self._bytes = sum(p.numel() * (3 * p.element_size() + (4 if self._is_8bit(p) else 16)) for p in ps)
+        moves = 3 if self.max_grad_norm is None else 4          # parameter read and written, gradient read -- twice for its norm
+        self._bytes = sum(p.numel() * (moves * p.element_size() + (4 if self._is_8bit(p) else 16)) for p in ps)
         return self._plan
 
     def _no_capture(self, what, how):
@@ -532,7 +533,7 @@ class FusedAdamW(torch.optim.Optimizer):
             table.holds, table.states = (ps, self._state_tensors(hp)), self._states_now()
             table.offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
             self._state_plan = {"key": key, "table": table, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "all": len(have) == len(ps),
-                                "layouts": list(map(self._state_layout, ps))}
+                                "layouts": list(map(self._state_layout, ps)), "bytes": sum(p.numel() * (10 if self._is_8bit(p) else 16) for p in hp)}
         return self._state_plan
 
     @torch.no_grad()
@@ -551,7 +552,7 @@ class FusedAdamW(torch.optim.Optimizer):
             if torch.cuda.is_current_stream_capturing():
                 self._kept.append((table.records, table.chunks, table.offsets, table.holds))
             if profiler.ACTIVE is not None:
-                profiler.note("adamw_moments", "hbm", 10.0 * total)
+                profiler.note("adamw_moments", "hbm", float(plan["bytes"]))
             call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
                  m.data_ptr(), v.data_ptr(), 0, stream)
         if flat:

@@ -464,3 +464,19 @@ def test_adamw_steps_without_gradients_are_not_forgotten(stubbed_adamw, monkeypa
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
     opt.load_state_dict(sd)                                     # what a checkpoint says counts
     assert opt.device_steps() == [8.0, 0.0, 0.0]
+
+
+def test_adamw_bytes_that_the_profiler_is_told(stubbed_adamw, monkeypatch):
+    from bts_amd import optim
+    notes = {}
+    monkeypatch.setattr(optim.profiler, "ACTIVE", object())
+    monkeypatch.setattr(optim.profiler, "note", lambda name, kind, work, *a: notes.update({name: work}))
+    for kw, step, moments in ((dict(state_bits=8), 5000 * 16 + 50 * 28 + 6000 * 10, 11000 * 10 + 50 * 16), (dict(state_bits=32), 5050 * 28 + 6000 * 22, 11050 * 16),
+                              (dict(state_bits=8, max_grad_norm=1.0), 5000 * 20 + 50 * 32 + 6000 * 12, 11000 * 10 + 50 * 16)):
+        ps = [torch.nn.Parameter(torch.zeros(n, dtype=t)) for n, t in ((5000, torch.float32), (50, torch.float32), (6000, torch.bfloat16), (7000, torch.float32))]
+        for p in ps[:3]:                                        # the last one has no gradient, no state and no part
+            p.grad = torch.zeros_like(p)
+        opt = optim.FusedAdamW(ps, **kw)
+        opt.step()
+        opt.moments()
+        assert notes == {"adamw_multi_step": step, "adamw_moments": moments}
