@@ -248,6 +248,8 @@ class FusedAdamW(torch.optim.Optimizer):
             _record([self._hyper, self._scratch, self._norm])
         if table is not None:
             table.use(stream)
+        if torch.cuda.is_current_stream_capturing():            # what a graph writes stays its own, whatever is made anew here
+            self._kept.append((self._hyper, self._scratch, self._norm) + (() if table is None else (table.records, table.chunks, table.offsets, table.holds)))
         return stream
 
     def _host_hyper(self, lrs=None):
@@ -549,8 +551,6 @@ class FusedAdamW(torch.optim.Optimizer):
         m, v = ((torch.empty if plan["all"] else torch.zeros)(total, dtype=torch.float32, device=self._device()) for _ in range(2))
         if table.n_chunks:
             stream = self._launch_on(table)
-            if torch.cuda.is_current_stream_capturing():
-                self._kept.append((table.records, table.chunks, table.offsets, table.holds))
             if profiler.ACTIVE is not None:
                 profiler.note("adamw_moments", "hbm", float(plan["bytes"]))
             call("bts_adamw_multi_moments", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, table.offsets.data_ptr(),
@@ -580,7 +580,7 @@ class FusedAdamW(torch.optim.Optimizer):
             return
         if torch.cuda.is_current_stream_capturing():
             # the memory itself: a parameter or gradient that is given other memory (p.data = ...) does not take this from the graph
-            self._kept.append((table.records, table.chunks, rows, table.holds, [t.detach() for p in table.holds[0] for t in (p, p.grad)]))
+            self._kept.append([t.detach() for p in table.holds[0] for t in (p, p.grad)])
         if profiler.ACTIVE is not None:
             profiler.note("adamw_multi_step", "hbm", float(self._bytes))
         call("bts_adamw_multi_step", table.records.data_ptr(), table.chunks.data_ptr(), table.n_chunks, rows.data_ptr(), len(self.param_groups), hyper,

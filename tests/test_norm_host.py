@@ -480,3 +480,18 @@ def test_adamw_bytes_that_the_profiler_is_told(stubbed_adamw, monkeypatch):
         opt.step()
         opt.moments()
         assert notes == {"adamw_multi_step": step, "adamw_moments": moments}
+
+
+def test_adamw_captured_work_keeps_the_device_rows(stubbed_adamw, monkeypatch):
+    """A captured step without gradients, or a captured prepare_step, writes the rows, too: add_param_group makes them anew."""
+    from bts_amd.optim import FusedAdamW
+    for use in (lambda o: o.step(prepared=True), lambda o: o.prepare_step()):
+        opt = FusedAdamW([torch.nn.Parameter(torch.zeros(50))], max_grad_norm=1.0)
+        opt.step()
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            use(opt)
+        rows, norm = opt._hyper.data_ptr(), opt._norm.data_ptr()
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
+        kept = {t.data_ptr() for k in opt._kept for t in k if torch.is_tensor(t)}
+        assert {rows, norm} <= kept
