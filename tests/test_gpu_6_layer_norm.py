@@ -427,3 +427,25 @@ def test_nearly_equal_elements_far_from_zero(C):
     # elements and mean are multiples of 2^-14 below 2^10: a difference of them is exact, but for the mean's correction, which adds up at
     # most 42 times (u each) and is at most 43 u 1000 itself; root, reciprocal, product
     assert ((y.double() - want).abs() <= 50 * U * (want.abs() + 43 * U * 1000 / 1e-5 ** 0.5)).all()
+
+
+# the kernel variants that SHAPES leaves out, and rows of odd width of which a block walks several (the next one is fetched ahead)
+F, B = torch.float32, torch.bfloat16
+MORE = [(F, 70, 4), (F, 65, 13), (F, 30, 200), (F, 31, 259), (F, 21, 640), (F, 19, 900), (F, 17, 1536), (F, 5, 9001), (F, 4, 12288), (B, 65, 11), (B, 30, 200),
+        (B, 31, 301), (B, 17, 1280), (B, 13, 1800), (B, 11, 2901), (B, 9, 3333), (B, 6, 4096),
+        (F, 9001, 201), (F, 9001, 301), (F, 9001, 667), (F, 5000, 1001), (F, 2100, 1401), (F, 1500, 2207), (F, 800, 8191), (F, 600, 9001), (F, 600, 16381),
+        (B, 40001, 41), (B, 9001, 301), (B, 9001, 667), (B, 3000, 1401), (B, 2500, 1801), (B, 2100, 2207), (B, 1500, 2901), (B, 1500, 3333), (B, 800, 8191), (B, 600, 9001)]
+
+
+@pytest.mark.parametrize("dtype,M,C", MORE)
+def test_forward_and_backward_of_every_variant(dtype, M, C):
+    x, w, b, dy = make(M, C, dtype, M * 37 + C)
+    y, stats = ops.layer_norm_fwd(x, w, b, 1e-5, want_stats=True)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, stats, w)
+    r = plain(x, w, b, 1e-5, dy)
+    within(y, r["y"], r["tol_y"], "y", HALF[dtype])
+    within(dx, r["dx"], r["tol_dx"], "dx", HALF[dtype])
+    within(dw, r["dw"], r["tol_dw"], "dweight")
+    within(db, r["db"], r["tol_db"], "dbias")
+    dx_only, _, _ = ops.layer_norm_bwd(dy, x, stats, w, True, False, False)
+    assert torch.equal(dx, dx_only)

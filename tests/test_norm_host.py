@@ -495,3 +495,31 @@ def test_adamw_captured_work_keeps_the_device_rows(stubbed_adamw, monkeypatch):
         opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
         kept = {t.data_ptr() for k in opt._kept for t in k if torch.is_tensor(t)}
         assert {rows, norm} <= kept
+
+
+def test_the_gpu_tests_reach_every_kernel():
+    """Forward and backward are compared with the definition for every variant (lanes, vectors a lane, odd widths), and with a block that
+    walks several rows for every variant of odd widths that has more than one vector a row."""
+    from tests.test_gpu_6_layer_norm import MORE, SHAPES
+
+    def variant(vec, c):                                        # the launcher's rule
+        nv = -(-c // vec)
+        most = 1 if nv <= 64 else (16 if c <= 1024 or c > 8192 else 8) // vec
+        lanes = 1
+        while lanes * most < nv:
+            lanes *= 2
+        if nv > 64:
+            lanes = 64 if c <= 1024 else -(-nv // 64) * 64 if vec == 8 and nv <= 384 else max(lanes, 256)
+        return lanes, -(-nv // lanes), c % vec != 0
+    for dtype, vec in ((torch.float32, 4), (torch.bfloat16, 8)):
+        cases = SHAPES + [(m, c) for t, m, c in MORE if t == dtype]
+        every = {variant(vec, c) for c in range(1, ops.LN_MAX_C + 1)}
+        assert every == {variant(vec, c) for _, c in cases}
+        walked = {}
+        for m, c in cases:
+            lanes, _, odd = variant(vec, c)
+            rows = 256 * (1024 // lanes if lanes > 64 else 4 * (256 // lanes))         # of a whole grid of the backward pass with sums
+            if odd and lanes >= 64 and m > rows:
+                walked[variant(vec, c)[:2]] = m
+        missing = {v[:2] for v in every if v[2] and v[0] >= 64} - set(walked)
+        assert not missing, (dtype, missing)
