@@ -4,7 +4,8 @@ The decoder normalises with BatchNorm (bts.py:155-172), whose statistics are tak
 not depend on the batch.  ``LayerNorm`` takes the place of ``torch.nn.LayerNorm`` (same arguments, parameters and state-dict keys),
 ``LayerNorm2d`` normalises the channels at every pixel of an NCHW map, where ``nn.BatchNorm2d`` would normalise the batch.
 
-Inputs are f32 or bf16, parameters and their gradients f32, statistics f32.  No second and no forward-mode derivatives, no
+Inputs are f32 or bf16, parameters and their gradients f32, statistics f32; the result has the input's type, also under autocast (where
+``torch.nn.LayerNorm`` gives f32 for a bf16 input), and ``module.bfloat16()`` makes parameters that are refused.  No second and no forward-mode derivatives, no
 torch.jit.trace (all refused), no CPU path.
 """
 import torch
@@ -75,7 +76,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 class LayerNorm(nn.LayerNorm):
-    """``torch.nn.LayerNorm`` on the HIP kernels: normalises over the trailing axes `normalized_shape`."""
+    """``torch.nn.LayerNorm`` on the HIP kernels: normalises over the trailing axes `normalized_shape`.  The result has x's type; the
+    parameters stay f32."""
 
     def forward(self, x):
         shape = tuple(self.normalized_shape)

@@ -449,3 +449,15 @@ def test_forward_and_backward_of_every_variant(dtype, M, C):
     within(db, r["db"], r["tol_db"], "dbias")
     dx_only, _, _ = ops.layer_norm_bwd(dy, x, stats, w, True, False, False)
     assert torch.equal(dx, dx_only)
+
+
+def test_the_result_has_the_inputs_type_under_autocast():
+    m = LayerNorm(40).to(DEV)
+    for x in (torch.randn(9, 40, device=DEV), torch.randn(9, 40, device=DEV).bfloat16()):
+        want = m(x)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = m(x)
+            y.float().square().sum().backward()
+        assert y.dtype == want.dtype == x.dtype and torch.equal(y, want) and m.weight.grad.dtype == torch.float32
+    with pytest.raises(BtsAmdError):
+        m.bfloat16()(x)
