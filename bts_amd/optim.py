@@ -43,7 +43,7 @@ optimizer keeps them: capture again after ``load_state_dict`` or ``add_param_gro
 import ctypes as C
 import itertools
 import math
-from operator import attrgetter, is_
+from operator import attrgetter, is_, itemgetter
 
 import numpy as np
 import torch
@@ -59,6 +59,7 @@ _RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("m_scal
 _RUN_FIRST = "run one step with the same parameters and gradients (zero_grad(set_to_none=False) keeps them)"
 _CODES = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")
 _ptr, _stride, _numel, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, torch.Tensor.numel, attrgetter("grad"), attrgetter("dtype")
+_params = itemgetter("params")
 
 
 def _dense(t):
@@ -437,13 +438,16 @@ class FusedAdamW(torch.optim.Optimizer):
         st = self.state.get(p)
         return _layout(p) if not st else st["layout"] if "layout" in st else _layout(st["exp_avg"])
 
+    def _parameters(self):
+        return list(itertools.chain.from_iterable(map(_params, self.param_groups)))
+
     def _states_now(self):
-        return self.state, list(self.state.values()), list(map(len, self.state.values()))
+        return self.state, list(self.state.values()), [st for st in self.state.values() if st]
 
     def _same_states(self, then):
         """The states are the dicts that they were, and none was emptied."""
-        state, dicts, lens = then
-        return self.state is state and len(state) == len(dicts) and all(map(is_, state.values(), dicts)) and list(map(len, dicts)) == lens
+        state, dicts, filled = then
+        return self.state is state and len(state) == len(dicts) and all(map(is_, state.values(), dicts)) and all(filled)
 
     def _records(self, ps, groups):
         """Rows of a device table, without the gradients' addresses: what the kernels go by is checked here."""
@@ -469,8 +473,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def _step_table(self):
         """The table of all parameters that have a gradient now.  What it was made from is compared every step: addresses, sizes and types of
         parameters and gradients and the gradients' strides; a gradient that moved costs one small upload, anything else a new table."""
-        ps = [p for g in self.param_groups for p in g["params"]]
-        lens, keep = [len(g["params"]) for g in self.param_groups], None
+        ps, lens, keep = self._parameters(), [len(g["params"]) for g in self.param_groups], None
         gs = list(map(_grad, ps))
         try:
             gptr = list(map(_ptr, gs))
@@ -523,32 +526,37 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _state_table(self):
         """The table of all parameters that have a state, for bts_adamw_multi_moments, and where each begins in flat moments."""
-        ps = [p for g in self.param_groups for p in g["params"]]
-        sizes = list(map(_numel, ps))
-        key = (list(map(id, ps)), sizes)
-        if self._state_plan is None or self._state_plan["key"] != key or not self._same_states(self._state_plan["table"].states):
+        ps, plan = self._parameters(), self._state_plan
+        if (plan is None or len(ps) != len(plan["all"]) or not all(map(is_, ps, plan["all"])) or not self._same_states(plan["table"].states)
+                or any(p.shape != shape for p, shape in plan["bare"])):
             self._no_capture("moments", "call moments() once")
-            offs = [0] + list(itertools.accumulate(sizes))
             have = [i for i, p in enumerate(ps) if self.state.get(p)]
-            hp = [ps[i] for i in have]
+            hp, layouts = [ps[i] for i in have], list(map(self._state_layout, ps))
+            sizes = [math.prod(shape) for shape, _ in layouts]
+            offs = [0] + list(itertools.accumulate(sizes))
             table = _Table(self._records(hp, [0] * len(hp)), [sizes[i] for i in have], self._device())
             table.holds, table.states = (ps, self._state_tensors(hp)), self._states_now()
             table.offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
-            self._state_plan = {"key": key, "table": table, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "all": len(have) == len(ps),
-                                "layouts": list(map(self._state_layout, ps)), "bytes": sum(p.numel() * (10 if self._is_8bit(p) else 16) for p in hp)}
+            self._state_plan = {"table": table, "all": ps, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "layouts": layouts,
+                                "bare": [(p, p.shape) for p in ps if not self.state.get(p)],           # without a state: zeros
+                                "bytes": sum(sizes[i] * (10 if "exp_avg_codes" in self.state[ps[i]] else 16) for i in have)}
         return self._state_plan
 
-    @torch.no_grad()
     def moments(self, flat=False):
         """What the states stand for, in f32: a list of (exp_avg, exp_avg_sq) per parameter in the groups' order, shaped like the parameters --
-        or, with flat, two vectors that hold them one after the other (each in the memory order that its parameter had when its state was made).  New memory every time;
-        zeros where a parameter has no state yet.  To be captured into a graph it must have been called once before."""
+        or, with flat, two vectors that hold them one after the other (each with the size and memory order that its parameter had when its state
+        was made).  New memory every time; zeros where a parameter has no state yet.  To be captured into a graph it must have been called once before."""
         if self._elsewhere() is not None:
             with torch.cuda.device(self._elsewhere()):
                 return self.moments(flat)
         plan = self._state_table()
+        if not flat:
+            for p, (shape, _) in zip(plan["all"], plan["layouts"]):
+                if p.shape != shape:
+                    raise BtsAmdError("FusedAdamW: a parameter is %s now, its state was made for %s" % (tuple(p.shape), tuple(shape)))
         table, total = plan["table"], plan["total"]
-        m, v = ((torch.empty if plan["all"] else torch.zeros)(total, dtype=torch.float32, device=self._device()) for _ in range(2))
+        new, dev = torch.zeros if plan["bare"] else torch.empty, self._device()
+        m, v = new(total, dtype=torch.float32, device=dev), new(total, dtype=torch.float32, device=dev)
         if table.n_chunks:
             stream = self._launch_on(table)
             if profiler.ACTIVE is not None:
@@ -606,15 +614,18 @@ class FusedAdamW(torch.optim.Optimizer):
         self._tables[gi] = (key, t)
         return t
 
-    @torch.no_grad()
     def step(self, closure=None, prepared=False):
         if closure is not None:
             raise BtsAmdError("FusedAdamW.step() does not support a closure (bts_main.py never passes one)")
-        if self._multi:
+        if self._multi:                 # (nothing there is an operation on a tensor that requires gradients)
             if self._elsewhere() is not None:
                 with torch.cuda.device(self._elsewhere()):
                     return self._step_multi(prepared)
             return self._step_multi(prepared)
+        return self._step_plain(prepared)
+
+    @torch.no_grad()
+    def _step_plain(self, prepared):
         if not prepared:
             self.prepare_step()
         rows = self._rows()

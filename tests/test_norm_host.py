@@ -425,6 +425,8 @@ def test_adamw_sees_that_states_were_reset(stubbed_adamw, bits):
     assert not any(a is b for a, b in zip(fourth, step()))
     opt.state.clear()
     assert all((t == 0).all() for mv in opt.moments() for t in mv) and not opt.state_dict()["state"]
+    ps[0].data = ps[0].data[:10]                                # a parameter without a state
+    assert [m.numel() for m, _ in opt.moments()] == [10, 50, 6000] and opt.moments(flat=True)[0].numel() == 6060
 
 
 def test_parameters_of_another_shape_are_refused_before_the_launch(monkeypatch):
