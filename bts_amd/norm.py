@@ -5,8 +5,8 @@ not depend on the batch.  ``LayerNorm`` takes the place of ``torch.nn.LayerNorm`
 ``LayerNorm2d`` normalises the channels at every pixel of an NCHW map, where ``nn.BatchNorm2d`` would normalise the batch.
 
 Inputs are f32 or bf16, parameters and their gradients f32, statistics f32; the result has the input's type, also under autocast (where
-``torch.nn.LayerNorm`` gives f32 for a bf16 input), and ``module.bfloat16()`` makes parameters that are refused.  No second and no forward-mode derivatives, no
-torch.jit.trace (all refused), no CPU path.
+``torch.nn.LayerNorm`` gives f32 for a bf16 input), and ``module.bfloat16()`` makes parameters that are refused.  No second and no
+forward-mode derivatives, no torch.jit.trace (all refused), no CPU path.
 """
 import torch
 import torch.autograd.forward_ad as forward_ad
