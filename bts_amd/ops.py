@@ -553,21 +553,21 @@ def layer_norm_bwd_unchecked(dy, dys, x, rows, stats, weight, want_dx, want_dwei
     """layer_norm_bwd for tensors whose layout is known: `rows`, `dys` = what row_stride says of x, of dy (its stride); x's device is the
     current one.  The autograd engine runs it on a thread of its own, where every line of Python costs three times what it costs here."""
     M, xs = rows
-    Cc, dt = x.shape[-1], dtype_code(x.dtype)
+    Cc, dt, dev = x.shape[-1], dtype_code(x.dtype), x.device
     dx = dw = db = ws = px = pw = pb = pws = None
     if want_dx:
-        dx = torch.empty_like(x) if xs == Cc else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = torch.empty_like(x) if xs == Cc else torch.empty(x.shape, dtype=x.dtype, device=dev)
         px = dx.data_ptr()
     if want_dweight:
-        dw = torch.empty(Cc, dtype=torch.float32, device=x.device)
+        dw = torch.empty(Cc, dtype=torch.float32, device=dev)
         pw = dw.data_ptr()
     if want_dbias:
-        db = torch.empty(Cc, dtype=torch.float32, device=x.device)
+        db = torch.empty(Cc, dtype=torch.float32, device=dev)
         pb = db.data_ptr()
     if not M:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     if want_dweight or want_dbias:
-        ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(call("bts_layernorm_bwd_workspace_bytes", dt, M, Cc), dtype=torch.uint8, device=dev)
         pws = ws.data_ptr()
     elif not want_dx:
         return None, None, None
