@@ -35,8 +35,8 @@ __device__ __forceinline__ u32x4_t drop_first(u32x4_t v, int n) {
 // A row's K vectors of one lane, as they are loaded: K - 1 whole ones, then one that may lie behind the row's end or, ODD (C is no multiple
 // of the vector), reach over it.  That one is loaded from where it still ends inside the row, so that no branch holds the loads up, and
 // settle() shifts it into place, zeros behind the row, when it is used.  Only rows shorter than a vector (one lane, one vector) go
-// element by element.  Stored in at most three pieces.  Against up to seven masked element accesses in every row, us forward /
-// backward: 20000 x 1001 bf16 24 / 54 -> 21 / 36, 8000 x 2207 bf16 32 / 75 -> 25 / 42, 20000 x 1001 f32 36 / 63 -> 35 / 55.
+// element by element.  Stored in at most three pieces.  Against up to seven masked element accesses in every row it takes off the
+// forward / backward pass: 20000 x 1001 bf16 12 / 33 %, 8000 x 2207 bf16 22 / 44 %, 20000 x 1001 f32 3 / 13 %.
 // AHEAD or not: where the row is used at once and C is a multiple of the vector, lanes behind the row's end skip their load instead (3344 x
 // 2208 f32, 472 idle lanes of 512 in the second vector: 0.8 us of 13 in the forward pass).
 template <typename T, int LANES, int K, bool ODD, bool AHEAD>
@@ -189,9 +189,11 @@ __device__ __forceinline__ void clear_sums(float* red) {                     // 
 // taken for every row regardless it costs rows near zero 71, 31, 44 and 14.3.
 constexpr float kFar = 16.f;
 
-// Bound by memory: 856064 x 96 bf16 63 us (5.2 TB/s; a large copy reaches 4.7-5.1), 8192 x 4096 f32 44 us (6.1, partly from the last-level
-// cache), 53504 x 128 f32 13.9 us, 418 x 512 bf16 3.3 us (launch and one latency).  Rows at odd addresses take two lines per vector:
-// 2000 x 8191 bf16 18.3 us, 3.6 TB/s.  Shared rows keep w and b in registers over the block's rows.
+// Bound by memory: 856064 x 96 bf16 64 us (5.1 TB/s; a large copy reaches 4.7-5.1), 8192 x 4096 f32 43.5 us (6.2, partly from the last-level
+// cache), 53504 x 128 f32 13.9 us, 418 x 512 bf16 3.1 us (launch and one latency), 2000 x 16384 bf16 27.4 us, f32 47 us.  Rows at odd
+// addresses, 2000 x 8191 bf16: 19.2 us, 3.4 TB/s.  The bytes from and to memory are those of even rows; the L1 counts 2.7 times the
+// accesses (backward 3.2 times), since it takes unaligned 16-byte vectors apart.  Shared rows keep w and b in registers over
+// the block's rows.
 // Rows of 1024 lanes are held to 64 registers where that spills nothing: two blocks a CU (2000 x 12288 bf16: 21 us, 26 at 68 registers).
 template <typename T, int LANES, int K, bool ODD>
 __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads, LANES == 1024 && !ODD ? 8 : 1) void ln_fwd_kernel(const void* __restrict__ x, long xs, void* __restrict__ y, long ys,
@@ -265,8 +267,11 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads, LANES == 1024 && !OD
     }
 }
 
-// 856064 x 96 bf16 102 us (4.8 TB/s) + 5 us for the final sums, 8192 x 4096 bf16 35 + 5, 3344 x 2208 f32 18.5 + 4.0, 13376 x 512 bf16
-// 9.6 + 3.9, 2000 x 8191 bf16 28 + 6, 418 x 512 bf16 3.6 + 3.4.
+// 856064 x 96 bf16 101 us (4.9 TB/s) + 5 us for the final sums, 8192 x 4096 bf16 35 + 4.5, 3344 x 2208 f32 19.2 + 4.0, 13376 x 512 bf16
+// 9.4 + 4.0, 2000 x 8191 bf16 28 + 6, 418 x 512 bf16 3.6 + 3.5, 4001 x 667 f32 9.2 + 6.1 (every block walks once and leaves its row of
+// sums: 5.3 MB written and read beside 32), 2000 x 16384 bf16 39 + 7, f32 83 + 7.
+// Registers with the sums: 64 lanes with two bf16 vectors or, odd, four f32 ones take 130 - 149, three waves a SIMD, so one of the four
+// blocks of a CU that the grid counts on waits; 1024 lanes with two bf16 vectors spill 2 (odd widths 8) of 128.
 // Every block walks rows in steps of the grid and keeps the sums of dy xh and dy over its rows in registers; it writes one partial row
 // [2][C] (ws), ln_bwd_final_kernel adds the rows in a fixed order: no atomics, the gradients of the parameters are reproducible.
 template <typename T, int LANES, int K, bool ODD, bool PARAM>
@@ -288,8 +293,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(c
     const float inv = 1.f / (float)C;
     const long step = (long)gridDim.x * RPB;
     long row = (long)blockIdx.x * RPB + threadIdx.x / LANES;
-    // bf16: the next row's vectors are on their way while this row's sums are taken (856064 x 96: 107 -> 95 us, 8192 x 4096: 53 -> 49).
-    // f32 has twice the bytes in flight as it is, and its raw vectors would cost twice the registers (8192 x 4096: 80 -> 83 us).
+    // bf16: the next row's vectors are on their way while this row's sums are taken (856064 x 96: 11 % of the pass, 8192 x 4096: 8 %).
+    // f32 has twice the bytes in flight as it is, and its raw vectors would cost twice the registers (8192 x 4096: 4 % longer).
     constexpr bool kAhead = T::kBytes == 2;
     u32x4_t xn[K], gn[K];
     float mun = 0.f, rsn = 0.f;
@@ -369,8 +374,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads) void ln_bwd_kernel(c
     }
 }
 
-// ws [rows][2][C] -> dw, db: 32 of the 2 C columns x 32 row lanes per block, combined in a fixed order (backward pass in all, us, at 16 /
-// 32 / 64 columns: 13376 x 512 bf16 13.8 / 12.9 / 14.3, 3344 x 2208 f32 21.1 / 19.4 / 20.0, 8192 x 4096 bf16 39.1 / 36.5 / 36.4).
+// ws [rows][2][C] -> dw, db: 32 of the 2 C columns x 32 row lanes per block, combined in a fixed order (16 or 64 columns make the whole
+// backward pass 7 or 11 % longer for 13376 x 512 bf16, 9 or 3 % for 3344 x 2208 f32, 7 or 0 % for 8192 x 4096 bf16).
 __global__ __launch_bounds__(1024) void ln_bwd_final_kernel(const float* __restrict__ ws, int rows, int C, float* __restrict__ dw, float* __restrict__ db) {
     constexpr int CL = 32, RL = 1024 / CL;
     __shared__ float part[RL][CL + 1];
@@ -401,11 +406,11 @@ constexpr int kLnMaxC = 16384;
 
 // Lanes of a row and vectors per lane.  A row of up to 64 vectors takes one vector per lane: neighbouring lanes read neighbouring 16
 // bytes and several rows share a wave.  Up to 64 lanes x 16 elements stay in one wave (no barrier), longer rows take a block at 8
-// elements per lane, and 16 above 8192 elements.  Both sides, forward / backward with its sums, us: 856064 x 96 bf16 16 x 1: 70 / 106,
-// 8 x 2: 71 / 102, 4 x 3: 95 / 166; 400000 x 32 f32 8 x 1: 20.3 / 32.6, 2 x 4: 26.3 / 44.5; 13376 x 512 bf16 64 x 1: 7.3 / 15.8,
-// 16 x 4: 34 / 59; 16384 x 1024 bf16 64 x 2: 14.8 / 27.7, 128 x 1: 15.7 / 32.9; 8192 x 4096 bf16 512 x 1: 28.3 / 52, 256 x 2: 31.6 / 58.
-// bf16 rows of 3, 5 or 6 waves take just those (20000 x 1025: 29.8 / 46 -> 26.2 / 42, 30000 x 2049: 83 / 134 -> 78 / 105); wider rows, and f32
-// with its two vectors per lane, do not gain by it (4000 x 5120 bf16 22.3 -> 25.6 / 29.6, 8000 x 2208 f32 28.0 / 44 -> 29.1 / 53).
+// elements per lane, and 16 above 8192 elements.  The other side against this one, time of the forward / backward pass with its sums:
+// 856064 x 96 bf16 16 lanes x 1: 8 x 2 1.01 / 0.96, 4 x 3 1.36 / 1.57; 400000 x 32 f32 8 x 1: 2 x 4 1.30 / 1.37; 13376 x 512 bf16 64 x 1:
+// 16 x 4 4.7 / 3.7; 16384 x 1024 bf16 64 x 2: 128 x 1 1.06 / 1.19; 8192 x 4096 bf16 512 x 1: 256 x 2 1.12 / 1.12.
+// bf16 rows of 3, 5 or 6 waves take just those (4, 8 and 8 instead: 20000 x 1025 1.14 / 1.10, 30000 x 2049 1.06 / 1.28); wider rows, and
+// f32 with its two vectors per lane, do not gain by it (4000 x 5120 bf16 1.15 - 1.33, 8000 x 2208 f32 1.04 / 1.20).
 static void ln_lanes(int V, int C, int& lanes, int& k) {
     const int nv = (C + V - 1) / V;
     int kmax = 1;
@@ -426,8 +431,9 @@ static LnPlan ln_plan(int dtype, long M, int C, int threads_per_cu) {
     return p;
 }
 // Threads per CU: all 2048 where nothing is summed over rows; half of them in the backward pass with the parameters' gradients, whose
-// blocks each leave a row of sums (us at 2048 / 1024 / 512: 856064 x 96 bf16 107 / 95 / 124, 3344 x 2208 f32 30 / 24 / 28; without
-// the sums 95 / 108 / 170 and 17.5 / 18.7 / 24).
+// blocks each leave a row of sums (2048 or 512 against 1024: 856064 x 96 bf16 1.13 or 1.31, 3344 x 2208 f32 1.25 or 1.17; without the
+// sums 1024 or 512 against 2048: 1.14 or 1.79, 1.07 or 1.37).  Both shapes walk several rows a block; fewer blocks for inputs whose
+// blocks would walk one were not tried.
 static LnPlan ln_fwd_plan(int dtype, long M, int C) { return ln_plan(dtype, M, C, 2048); }
 static LnPlan ln_bwd_plan(int dtype, long M, int C, bool sums) { return ln_plan(dtype, M, C, sums ? 1024 : 2048); }
 

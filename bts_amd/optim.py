@@ -91,6 +91,11 @@ def _layout(t):
     return t.size(), t.stride()
 
 
+def _layout_of(st, p):
+    """Shape and order in memory that p's state `st` was made for."""
+    return _layout(p) if not st else st["layout"] if "layout" in st else _layout(st["exp_avg"])
+
+
 def _like(flat, off, layout):
     """The elements of `flat` from `off` on, with the shape and order in memory of _layout(p)."""
     return torch.as_strided(flat, *layout, flat.storage_offset() + off)
@@ -119,12 +124,14 @@ class _Table:
         self.records = pinned.to(device, non_blocking=True)
         self.records_on = raw_stream()
 
-    def use(self, stream):
+    def use(self, stream, states_on):
         """Called before a launch on `stream`, the current one: memory that the allocator gave to another one must outlive this one's work
         -- the tables, and the states that the launch writes, also where the optimizer drops them while it runs."""
         if stream not in self.used_on:
             self.used_on.add(stream)
-            _record([self.chunks, self.offsets] + list({t.untyped_storage().data_ptr(): t for t in self.holds[1] if t.numel()}.values()))
+            _record([self.chunks, self.offsets])
+            if states_on != {stream}:
+                _record({t.untyped_storage().data_ptr(): t for t in self.holds[1] if t.numel()}.values())
         if stream != self.records_on:
             _record([self.records])
 
@@ -147,6 +154,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._options = (state_bits or 32, int(min_8bit_size), None if max_grad_norm is None else float(max_grad_norm))
         self._multi = state_bits is not None or max_grad_norm is not None
         self._forget()
+        self._states_on = set()
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
 
@@ -163,6 +171,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._kept = []             # what captured graphs refer to
         self._scratch = self._norm = None
         self._used_on = set()       # streams that _hyper, _scratch and _norm are recorded for
+        self._states_on = {None}    # streams that the states were allocated on; None: who knows
 
     def __getstate__(self):         # copies and pickles: states with their step counts, nothing that holds addresses
         self._refresh_steps()
@@ -183,7 +192,7 @@ class FusedAdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         self._seen = None
         if not self._multi and any(p.dtype != torch.float32 for p in self.param_groups[-1]["params"]):
-            self._multi, self._tables = True, {}
+            self._multi, self._tables, self._states_on = True, {}, {None}
 
     # ---- device-resident schedule / step counter ------------------------------------------------
     def _device(self):
@@ -248,7 +257,7 @@ class FusedAdamW(torch.optim.Optimizer):
             self._used_on.add(stream)
             _record([self._hyper, self._scratch, self._norm])
         if table is not None:
-            table.use(stream)
+            table.use(stream, self._states_on)
         if torch.cuda.is_current_stream_capturing():            # what a graph writes stays its own, whatever is made anew here
             self._kept.append((self._hyper, self._scratch, self._norm) + (() if table is None else (table.records, table.chunks, table.offsets, table.holds)))
         return stream
@@ -373,6 +382,7 @@ class FusedAdamW(torch.optim.Optimizer):
         ps = [p for g in self.param_groups for p in g["params"]]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         self.state.clear()
+        self._states_on = set()
         todo = [(p, state_dict["state"][i]) for i, p in zip(ids, ps) if state_dict["state"].get(i)]
         if not todo:
             return
@@ -414,6 +424,7 @@ class FusedAdamW(torch.optim.Optimizer):
         """Zero states for parameters that have none: one allocation for all codes, one for all scales, one for all f32 moments."""
         eight, wide = [p for p in ps if self._is_8bit(p)], [p for p in ps if not self._is_8bit(p)]
         dev = self._device()
+        self._states_on.add(raw_stream())
         blocks = [-(-p.numel() // _BLOCK) for p in eight]
         codes = torch.zeros((2, sum(blocks) * _BLOCK), dtype=torch.uint8, device=dev)
         scales = torch.full((2, sum(blocks)), 2.0 ** -126, dtype=torch.float32, device=dev)
@@ -433,11 +444,6 @@ class FusedAdamW(torch.optim.Optimizer):
     def _state_tensors(self, ps):
         return [t for p in ps for k, t in self.state[p].items() if k not in ("step", "layout")]
 
-    def _state_layout(self, p):
-        """Shape and order in memory that p's state was made for."""
-        st = self.state.get(p)
-        return _layout(p) if not st else st["layout"] if "layout" in st else _layout(st["exp_avg"])
-
     def _parameters(self):
         return list(itertools.chain.from_iterable(map(_params, self.param_groups)))
 
@@ -449,11 +455,17 @@ class FusedAdamW(torch.optim.Optimizer):
         state, dicts, filled = then
         return self.state is state and len(state) == len(dicts) and all(map(is_, state.values(), dicts)) and all(filled)
 
-    def _records(self, ps, groups):
-        """Rows of a device table, without the gradients' addresses: what the kernels go by is checked here."""
+    def _records(self, ps, groups, as_now):
+        """Rows of a device table, without the gradients' addresses: what the kernels go by is checked here.  as_now: the states must have
+        been made for the shape and the order in memory that the parameters have now."""
         rows = []
         for p, gi in zip(ps, groups):
             st, n = self.state[p], p.numel()
+            if as_now:
+                shape, strides = _layout_of(st, p)
+                if shape != p.shape or not _same_strides(strides, p.stride(), shape):
+                    raise BtsAmdError("FusedAdamW: a parameter is %s with strides %s now, its state was made for %s with strides %s -- "
+                                      "load_state_dict(state_dict()) makes it anew" % (tuple(p.shape), p.stride(), tuple(shape), strides))
             flags = _BF16 if p.dtype == torch.bfloat16 else 0
             if "exp_avg_codes" in st:
                 a, sa, b, sb = (st[k] for k in _CODES)
@@ -506,12 +518,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if fresh:
             self._new_state(fresh)
             self._state_plan = None
-        for p in ps:
-            shape, strides = self._state_layout(p)
-            if shape != p.shape or not _same_strides(strides, p.stride(), shape):
-                raise BtsAmdError("FusedAdamW: a parameter is %s with strides %s now, its state was made for %s with strides %s -- load_state_dict(state_dict()) "
-                                  "makes it anew" % (tuple(p.shape), p.stride(), tuple(shape), strides))
-        rec = self._records(ps, groups)
+        rec = self._records(ps, groups, True)
         rec["g"] = gptr
         self._plan = _Table(rec, [p.numel() for p in ps], self._device())
         self._plan.holds, self._plan.states = (ps, self._state_tensors(ps)), self._states_now()     # the addresses in the table stay theirs
@@ -531,10 +538,10 @@ class FusedAdamW(torch.optim.Optimizer):
                 or any(p.shape != shape for p, shape in plan["bare"])):
             self._no_capture("moments", "call moments() once")
             have = [i for i, p in enumerate(ps) if self.state.get(p)]
-            hp, layouts = [ps[i] for i in have], list(map(self._state_layout, ps))
+            hp, layouts = [ps[i] for i in have], [_layout_of(self.state.get(p), p) for p in ps]
             sizes = [math.prod(shape) for shape, _ in layouts]
             offs = [0] + list(itertools.accumulate(sizes))
-            table = _Table(self._records(hp, [0] * len(hp)), [sizes[i] for i in have], self._device())
+            table = _Table(self._records(hp, [0] * len(hp), False), [sizes[i] for i in have], self._device())
             table.holds, table.states = (ps, self._state_tensors(hp)), self._states_now()
             table.offsets = torch.tensor([offs[i] for i in have], dtype=torch.int64).to(self._device())
             self._state_plan = {"table": table, "all": ps, "at": dict(zip(map(id, ps), offs)), "total": offs[-1], "layouts": layouts,
