@@ -59,6 +59,7 @@ _RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("m_scal
 _RUN_FIRST = "run one step with the same parameters and gradients (zero_grad(set_to_none=False) keeps them)"
 _CODES = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")
 _ptr, _stride, _numel, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, torch.Tensor.numel, attrgetter("grad"), attrgetter("dtype")
+_contiguous = torch.Tensor.is_contiguous
 _params = itemgetter("params")
 
 
@@ -495,8 +496,9 @@ class FusedAdamW(torch.optim.Optimizer):
             gptr = list(map(_ptr, gs))
         if not ps:
             return None
-        seen = (lens, keep, list(map(_ptr, ps)), list(map(_numel, ps)), list(map(_dtype, gs)), list(map(_stride, gs)))
-        if self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])) and self._same_states(self._plan.states):
+        seen = (lens, keep, list(map(_ptr, ps)), list(map(_numel, ps)), list(map(_dtype, gs)))
+        if (self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])) and self._same_states(self._plan.states)
+                and (all(map(_contiguous, gs)) if self._strides is None else list(map(_stride, gs)) == self._strides)):
             if gptr == self._gptr:
                 return self._plan
             if list(map(_numel, gs)) == seen[3]:
@@ -523,6 +525,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self._plan = _Table(rec, [p.numel() for p in ps], self._device())
         self._plan.holds, self._plan.states = (ps, self._state_tensors(ps)), self._states_now()     # the addresses in the table stay theirs
         self._seen, self._gptr = seen, gptr
+        self._strides = None if all(map(_contiguous, gs)) else list(map(_stride, gs))
         moves = 3 if self.max_grad_norm is None else 4          # parameter read and written, gradient read -- twice for its norm
         self._bytes = sum(p.numel() * (moves * p.element_size() + (4 if self._is_8bit(p) else 16)) for p in ps)
         return self._plan
