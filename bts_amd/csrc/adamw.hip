@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const bts_adamw_tensor
 }
 
 // sum of squares of every gradient, in f64 (no overflow of g^2, no loss over 10^8 terms): one partial sum per block, fixed order.
-// 1000 M f32 gradients: 712 us, 5.6 TB/s; 112.8 M: 53 us, more than memory gives, since a part is in the last-level cache still.
+// 1000 M f32 gradients: 710 us, 5.6 TB/s; 112.8 M: 53 us, more than memory gives, since a part is in the last-level cache still.
 template <bool BF>
 __device__ __forceinline__ void add_squares(const bts_adamw_tensor_t& t, long base, double& s) {
     Raw4<BF> r[4];

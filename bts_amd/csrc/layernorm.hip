@@ -190,8 +190,8 @@ __device__ __forceinline__ void clear_sums(float* red) {                     // 
 constexpr float kFar = 16.f;
 
 // Bound by memory: 856064 x 96 bf16 64 us (5.1 TB/s; a large copy reaches 4.7-5.1), 8192 x 4096 f32 43.5 us (6.2, partly from the last-level
-// cache), 53504 x 128 f32 13.9 us, 418 x 512 bf16 3.1 us (launch and one latency), 2000 x 16384 bf16 27.4 us, f32 47 us.  Rows at odd
-// addresses, 2000 x 8191 bf16: 19.2 us, 3.4 TB/s.  The bytes from and to memory are those of even rows; the L1 counts 2.7 times the
+// cache), 53504 x 128 f32 13.2 us, 418 x 512 bf16 3.0 us (launch and one latency), 2000 x 16384 bf16 27.4 us, f32 47 us.  Rows at odd
+// addresses, 2000 x 8191 bf16: 19.5 us, 3.4 TB/s.  The bytes from and to memory are those of even rows; the L1 counts 2.7 times the
 // accesses (backward 3.2 times), since it takes unaligned 16-byte vectors apart.  Shared rows keep w and b in registers over
 // the block's rows.
 // Rows of 1024 lanes are held to 64 registers where that spills nothing: two blocks a CU (2000 x 12288 bf16: 21 us, 26 at 68 registers).
@@ -267,9 +267,9 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : kThreads, LANES == 1024 && !OD
     }
 }
 
-// 856064 x 96 bf16 101 us (4.9 TB/s) + 5 us for the final sums, 8192 x 4096 bf16 35 + 4.5, 3344 x 2208 f32 19.2 + 4.0, 13376 x 512 bf16
-// 9.4 + 4.0, 2000 x 8191 bf16 28 + 6, 418 x 512 bf16 3.6 + 3.5, 4001 x 667 f32 9.2 + 6.1 (every block walks once and leaves its row of
-// sums: 5.3 MB written and read beside 32), 2000 x 16384 bf16 39 + 7, f32 83 + 7.
+// 856064 x 96 bf16 102 us (4.8 TB/s) + 5 us for the final sums, 8192 x 4096 bf16 35.6 + 4.8, 3344 x 2208 f32 17.4 + 3.9, 13376 x 512 bf16
+// 9.8 + 3.8, 2000 x 8191 bf16 27 + 6, 418 x 512 bf16 3.5 + 3.4, 4001 x 667 f32 9.2 + 5.7 (every block walks once and leaves its row of
+// sums: 5.3 MB written and read beside 32), 2000 x 16384 bf16 40 + 7, f32 83 + 7.
 // Registers with the sums: 64 lanes with two bf16 vectors or, odd, four f32 ones take 130 - 149, three waves a SIMD, so one of the four
 // blocks of a CU that the grid counts on waits; 1024 lanes with two bf16 vectors spill 2 (odd widths 8) of 128.
 // Every block walks rows in steps of the grid and keeps the sums of dy xh and dy over its rows in registers; it writes one partial row

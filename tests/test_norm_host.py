@@ -525,3 +525,21 @@ def test_the_gpu_tests_reach_every_kernel():
                 walked[variant(vec, c)[:2]] = m
         missing = {v[:2] for v in every if v[2] and v[0] >= 64} - set(walked)
         assert not missing, (dtype, missing)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_a_reset_state_takes_the_parameters_new_shape(stubbed_adamw, bits):
+    from bts_amd.optim import FusedAdamW
+    p, q = torch.nn.Parameter(torch.zeros(9000)), torch.nn.Parameter(torch.zeros(50))
+    opt = FusedAdamW([p, q], state_bits=bits)
+    p.grad, q.grad = torch.zeros(9000), torch.zeros(50)
+    opt.step()
+    opt.moments()
+    p.data, p.grad = p.data[:5000], None
+    p.grad = torch.zeros(5000)
+    with pytest.raises(_lib.BtsAmdError):
+        opt.step()
+    opt.state[p] = {}
+    opt.step()
+    assert stubbed_adamw[-1][1]["n"].tolist() == [5000, 50] and [m.numel() for m, _ in opt.moments()] == [5000, 50]
+    assert opt.moments(flat=True)[0].numel() == 5050 and stubbed_adamw[-1][1]["n"].tolist() == [5000, 50]
