@@ -59,8 +59,7 @@ _RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("m_scal
 _RUN_FIRST = "run one step with the same parameters and gradients (zero_grad(set_to_none=False) keeps them)"
 _CODES = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")
 _ptr, _stride, _numel, _grad, _dtype = torch.Tensor.data_ptr, torch.Tensor.stride, torch.Tensor.numel, attrgetter("grad"), attrgetter("dtype")
-_contiguous = torch.Tensor.is_contiguous
-_params = itemgetter("params")
+_contiguous, _params = torch.Tensor.is_contiguous, itemgetter("params")
 
 
 def _dense(t):
@@ -113,7 +112,7 @@ class _Table:
         chunks[:, 1] = np.arange(self.n_chunks) - np.repeat(np.cumsum(counts) - counts, counts)
         self.host = records
         self.holds = self.offsets = None        # what must live as long as the addresses; begin of each tensor in flat moments
-        self.states = None                      # _states_now() when it was made
+        self.states = self.shaped = None        # _states_now() when it was made; the parameters that have an order in memory
         self.chunks = torch.from_numpy(chunks).to(device)
         self.records = torch.from_numpy(records.view(np.uint8)).to(device)
         self.records_on, self.used_on = raw_stream(), set()
@@ -236,19 +235,19 @@ class FusedAdamW(torch.optim.Optimizer):
         """The device rows, created on first use from the groups' hyper-parameters and recorded state."""
         if self._hyper is None:
             self._used_on = set()
-            steps, self._steps = self._group_steps(), None
+            steps = self._group_steps()
             if self._multi:
                 rows = np.zeros((len(self.param_groups) + 1, _WIDE_ROW))
                 for r, g, t in zip(rows, self.param_groups, steps):
                     r[0], r[3], r[4:6], r[6], r[7] = float(g["lr"]), t, g["betas"], g["eps"], g["weight_decay"]
                 rows[-1, 0] = math.inf if self.max_grad_norm is None else self.max_grad_norm
-                self._hyper = torch.from_numpy(rows).to(self._device())
+                self._hyper, self._steps = torch.from_numpy(rows).to(self._device()), None
                 return self._hyper
             rows = []
             for g, t in zip(self.param_groups, steps):
                 b1, b2 = g["betas"]
                 rows.append([float(g["lr"]), 1.0, 1.0, t, float(b1), float(b2), 0.0, 0.0])
-            self._hyper = torch.tensor(rows, dtype=torch.float32).to(self._device())
+            self._hyper, self._steps = torch.tensor(rows, dtype=torch.float32).to(self._device()), None
         return self._hyper
 
     def _launch_on(self, table=None):
@@ -448,6 +447,12 @@ class FusedAdamW(torch.optim.Optimizer):
     def _parameters(self):
         return list(itertools.chain.from_iterable(map(_params, self.param_groups)))
 
+    def _same_order(self, gs):
+        """Parameters and gradients lie in memory as they did when the step's table was made (strides: only where some are not contiguous)."""
+        if self._order is not None:
+            return list(map(_stride, gs)) == self._order
+        return all(map(_contiguous, gs)) and all(map(_contiguous, self._plan.shaped))
+
     def _states_now(self):
         return self.state, list(self.state.values()), [st for st in self.state.values() if st]
 
@@ -462,11 +467,12 @@ class FusedAdamW(torch.optim.Optimizer):
         rows = []
         for p, gi in zip(ps, groups):
             st, n = self.state[p], p.numel()
-            if as_now:
-                shape, strides = _layout_of(st, p)
-                if shape != p.shape or not _same_strides(strides, p.stride(), shape):
+            made, now = _layout_of(st, p), _layout(p)
+            if as_now and made != now:
+                (shape, strides), here = made, now[1]
+                if shape != p.shape or not _same_strides(strides, here, shape):
                     raise BtsAmdError("FusedAdamW: a parameter is %s with strides %s now, its state was made for %s with strides %s -- "
-                                      "load_state_dict(state_dict()) makes it anew" % (tuple(p.shape), p.stride(), tuple(shape), strides))
+                                      "load_state_dict(state_dict()) makes it anew" % (tuple(p.shape), here, tuple(shape), strides))
             flags = _BF16 if p.dtype == torch.bfloat16 else 0
             if "exp_avg_codes" in st:
                 a, sa, b, sb = (st[k] for k in _CODES)
@@ -498,7 +504,7 @@ class FusedAdamW(torch.optim.Optimizer):
             return None
         seen = (lens, keep, list(map(_ptr, ps)), list(map(_numel, ps)), list(map(_dtype, gs)))
         if (self._plan is not None and seen == self._seen and all(map(is_, ps, self._plan.holds[0])) and self._same_states(self._plan.states)
-                and (all(map(_contiguous, gs)) if self._strides is None else list(map(_stride, gs)) == self._strides)):
+                and self._same_order(gs)):
             if gptr == self._gptr:
                 return self._plan
             if list(map(_numel, gs)) == seen[3]:
@@ -524,8 +530,10 @@ class FusedAdamW(torch.optim.Optimizer):
         rec["g"] = gptr
         self._plan = _Table(rec, [p.numel() for p in ps], self._device())
         self._plan.holds, self._plan.states = (ps, self._state_tensors(ps)), self._states_now()     # the addresses in the table stay theirs
-        self._seen, self._gptr = seen, gptr
-        self._strides = None if all(map(_contiguous, gs)) else list(map(_stride, gs))
+        self._plan.shaped = [p for p in ps if p.dim() > 1]
+        self._seen, self._gptr, self._order = seen, gptr, None
+        if not all(map(_contiguous, itertools.chain(ps, gs))):
+            self._order = list(map(_stride, gs))
         moves = 3 if self.max_grad_norm is None else 4          # parameter read and written, gradient read -- twice for its norm
         self._bytes = sum(p.numel() * (moves * p.element_size() + (4 if self._is_8bit(p) else 16)) for p in ps)
         return self._plan

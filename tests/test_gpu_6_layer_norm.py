@@ -461,3 +461,22 @@ def test_the_result_has_the_inputs_type_under_autocast():
         assert y.dtype == want.dtype == x.dtype and torch.equal(y, want) and m.weight.grad.dtype == torch.float32
     with pytest.raises(BtsAmdError):
         m.bfloat16()(x)
+
+
+def test_checkpointed_and_offloaded_passes():
+    """A slice of a wider buffer through torch.utils.checkpoint, whose recomputed tensors take the saved ones' place."""
+    from torch.utils.checkpoint import checkpoint
+    x, w, b, dy = make(300, 96, torch.float32, 97, pad=7)
+    x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+
+    def block(x):
+        return layer_norm(torch.relu(layer_norm(x, w, b)) * 2, w, b)
+    want = torch.autograd.grad(block(x), (x, w, b), dy)
+    for reentrant in (True, False):
+        got = []
+        for t in (x, w, b):
+            t.grad = None
+        block_out = checkpoint(block, x, use_reentrant=reentrant)
+        block_out.backward(dy)
+        got = [t.grad for t in (x, w, b)]
+        assert all(torch.equal(a, c) for a, c in zip(got, want))

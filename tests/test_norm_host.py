@@ -543,3 +543,19 @@ def test_adamw_a_reset_state_takes_the_parameters_new_shape(stubbed_adamw, bits)
     opt.step()
     assert stubbed_adamw[-1][1]["n"].tolist() == [5000, 50] and [m.numel() for m, _ in opt.moments()] == [5000, 50]
     assert opt.moments(flat=True)[0].numel() == 5050 and stubbed_adamw[-1][1]["n"].tolist() == [5000, 50]
+
+
+def test_adamw_sees_a_parameter_transposed_in_place(stubbed_adamw):
+    """p.data = p.data.t() keeps address and size; a contiguous gradient of the new shape lies in another order."""
+    from bts_amd.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(60, 80))
+    opt = FusedAdamW([p], state_bits=8, min_8bit_size=1)
+    p.grad = torch.zeros(60, 80)
+    opt.step()
+    p.data, p.grad = p.data.t(), None
+    n = len(stubbed_adamw)
+    for grad in (torch.zeros(80, 60), torch.zeros(60, 80).t()):
+        p.grad = grad
+        with pytest.raises(_lib.BtsAmdError):
+            opt.step()
+    assert len(stubbed_adamw) == n
