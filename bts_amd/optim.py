@@ -386,10 +386,10 @@ class FusedAdamW(torch.optim.Optimizer):
         todo = [(p, state_dict["state"][i]) for i, p in zip(ids, ps) if state_dict["state"].get(i)]
         if not todo:
             return
-        self._new_state([p for p, _ in todo])
-        for p, st in todo:
-            self.state[p]["step"] = torch.as_tensor(st["step"], dtype=torch.float32).reshape(()).cpu().clone()
         with torch.cuda.device(self._device()):
+            self._new_state([p for p, _ in todo])
+            for p, st in todo:
+                self.state[p]["step"] = torch.as_tensor(st["step"], dtype=torch.float32).reshape(()).cpu().clone()
             plan = self._state_table()
             table = plan["table"]
             m = torch.empty(plan["total"], dtype=torch.float32, device=self._device())
@@ -468,11 +468,9 @@ class FusedAdamW(torch.optim.Optimizer):
         for p, gi in zip(ps, groups):
             st, n = self.state[p], p.numel()
             made, now = _layout_of(st, p), _layout(p)
-            if as_now and made != now:
-                (shape, strides), here = made, now[1]
-                if shape != p.shape or not _same_strides(strides, here, shape):
-                    raise BtsAmdError("FusedAdamW: a parameter is %s with strides %s now, its state was made for %s with strides %s -- "
-                                      "load_state_dict(state_dict()) makes it anew" % (tuple(p.shape), here, tuple(shape), strides))
+            if as_now and made != now and (made[0] != now[0] or not _same_strides(made[1], now[1], now[0])):
+                raise BtsAmdError("FusedAdamW: a parameter is %s with strides %s now, its state was made for %s with strides %s -- "
+                                  "load_state_dict(state_dict()) makes it anew" % (tuple(now[0]), now[1], tuple(made[0]), made[1]))
             flags = _BF16 if p.dtype == torch.bfloat16 else 0
             if "exp_avg_codes" in st:
                 a, sa, b, sb = (st[k] for k in _CODES)
