@@ -371,7 +371,7 @@ class FusedAdamW(torch.optim.Optimizer):
             self._one_step({float(st["step"]) for _, _, st in there if "step" in st})
             todo += there
         for i, p, st in todo:
-            if "step" not in st or any(k not in st or tuple(st[k].shape) != tuple(p.shape) for k in ("exp_avg", "exp_avg_sq")):
+            if self._multi and "step" not in st or any(k not in st or tuple(st[k].shape) != tuple(p.shape) for k in ("exp_avg", "exp_avg_sq")):
                 raise BtsAmdError("FusedAdamW.load_state_dict: parameter %r needs step, and exp_avg and exp_avg_sq of shape %s" % (i, tuple(p.shape)))
         if self._multi and todo:
             self._check_parameters([p for _, p, _ in todo])

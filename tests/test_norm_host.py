@@ -374,7 +374,8 @@ def test_adamw_a_refused_checkpoint_changes_nothing(stubbed_adamw, kw):
     had = {id(t): {k: v for k, v in st.items()} for t, st in opt.state.items()}
     hyper = opt._hyper
     bads = [lambda sd: sd["state"][1].update(step=torch.tensor(7.0))]
-    bads += [lambda sd: sd["state"][1].update(exp_avg=torch.zeros(3)), lambda sd: sd["state"][0].pop("exp_avg_sq"), lambda sd: sd["state"][1].pop("step")]
+    bads += [lambda sd: sd["state"][1].update(exp_avg=torch.zeros(3)), lambda sd: sd["state"][0].pop("exp_avg_sq")]
+    bads += [lambda sd: sd["state"][1].pop("step")] if kw else []
     for bad in bads:
         sd = copy.deepcopy(good)
         sd["param_groups"][0]["lr"] = 0.25
