@@ -393,7 +393,7 @@ def test_saved_tensor_hooks_may_change_the_layout(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("C", [1, 3, 7, 41, 200, 257, 667, 1025, 2208, 2900, 4097, 8191, 9001, 16384])
+@pytest.mark.parametrize("C", [1, 3, 7, 13, 30, 41, 100, 200, 257, 667, 1025, 2208, 2900, 4097, 8191, 9001, 16384])
 def test_rows_of_equal_elements_are_centred_exactly(C, dtype):
     """Variance 0, whatever the value and the width.  Far from zero (|mean| > 4 sqrt(eps)) y is the bias and the mean is the value, bit for
     bit, and the weight's gradient is 0; below, and for the statistics of what is left there, the tolerances of any row hold."""
