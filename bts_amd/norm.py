@@ -34,8 +34,9 @@ def _backward(ctx, dy):
     x, weight = ctx.saved_tensors
     need = ctx.needs_input_grad
     dy, (_, dys) = _rows(dy)
-    if x.stride() == ctx.strides and x.shape == dy.shape and x.dtype == dy.dtype and (
-            weight is None or weight.dtype == torch.float32 and weight.is_contiguous() and weight.numel() == x.shape[-1]):
+    dev = dy.get_device()
+    if x.stride() == ctx.strides and x.shape == dy.shape and x.dtype == dy.dtype and x.get_device() == dev and (
+            weight is None or weight.dtype == torch.float32 and weight.is_contiguous() and weight.numel() == x.shape[-1] and weight.get_device() == dev):
         return (*ops.layer_norm_bwd_unchecked(dy, dys, x, ctx.rows, ctx.stats, weight, need[0], need[1], need[2]), None)
     # Saved-tensor hooks gave back other tensors than were saved (save_on_cpu: a slice of a wider buffer comes back dense): their own
     # layout counts, and what is not the saved values' shape, type and device is refused.

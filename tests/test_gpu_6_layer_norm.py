@@ -480,3 +480,14 @@ def test_checkpointed_and_offloaded_passes():
         block_out.backward(dy)
         got = [t.grad for t in (x, w, b)]
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_saved_tensors_that_come_back_elsewhere_are_refused():
+    """A hook that moves what is saved to the host and leaves it there: refused, the kernel must not see host memory."""
+    x, w, b, dy = make(40, 64, torch.float32, 101)
+    for only in (x, w):
+        x, w, b = (t.detach().requires_grad_(True) for t in (x, w, b))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu() if t.shape == only.shape else t, lambda t: t):
+            y = layer_norm(x, w, b)
+        with pytest.raises(BtsAmdError):
+            torch.autograd.grad(y, (x, w, b), dy)

@@ -559,3 +559,27 @@ def test_adamw_sees_a_parameter_transposed_in_place(stubbed_adamw):
         with pytest.raises(_lib.BtsAmdError):
             opt.step()
     assert len(stubbed_adamw) == n
+
+
+def test_backward_refuses_what_comes_back_on_another_device(stubbed_norm, monkeypatch):
+    """(Stand-ins for a GPU: the gradient claims device 0, and so does what the forward pass saved.)"""
+    moved, keep = set(), []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: -1 if t.data_ptr() in moved else 0)
+    monkeypatch.setattr(ops, "current_device", lambda: 0)
+
+    def refuse(t):
+        raise _lib.BtsAmdError("not on a GPU")
+    monkeypatch.setattr(_lib, "require_gpu", refuse)
+
+    def move(t):
+        keep.append(t.clone())
+        moved.add(keep[-1].data_ptr())
+        return keep[-1]
+    for only in ((8, 16), (16,)):
+        x, w = torch.randn(8, 16, requires_grad=True), torch.ones(16, requires_grad=True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: move(t) if t.shape == only else t):
+            y = layer_norm(x, w)
+        n = len(stubbed_norm)
+        with pytest.raises(_lib.BtsAmdError):
+            y.sum().backward()
+        assert len(stubbed_norm) == n
