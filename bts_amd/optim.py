@@ -475,6 +475,7 @@ class FusedAdamW(torch.optim.Optimizer):
             if "exp_avg_codes" in st:
                 a, sa, b, sb = (st[k] for k in _CODES)
                 if not (a.dtype == b.dtype == torch.uint8 and sa.dtype == sb.dtype == torch.float32 and a.is_contiguous() and b.is_contiguous()
+                        and sa.is_contiguous() and sb.is_contiguous() and a.device == b.device == sa.device == sb.device == p.device
                         and a.data_ptr() % 4 == 0 and b.data_ptr() % 4 == 0 and a.numel() == b.numel() == n
                         and sa.numel() == sb.numel() == -(-n // _BLOCK) and _room(a) >= sa.numel() * _BLOCK and _room(b) >= sa.numel() * _BLOCK):
                     raise BtsAmdError("FusedAdamW: the 8-bit state of a parameter of %d elements was replaced by something else, or is one of %d elements" % (n, a.numel()))

@@ -583,3 +583,20 @@ def test_backward_refuses_what_comes_back_on_another_device(stubbed_norm, monkey
         with pytest.raises(_lib.BtsAmdError):
             y.sum().backward()
         assert len(stubbed_norm) == n
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_refuses_states_on_another_device(stubbed_adamw, bits):
+    """An optimizer whose state tensors were moved off the device: a new table must not take their addresses."""
+    from bts_amd.optim import FusedAdamW
+    for k in (("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales") if bits == 8 else ("exp_avg", "exp_avg_sq")):
+        p = torch.nn.Parameter(torch.zeros(9000))
+        opt = FusedAdamW([p], state_bits=bits)
+        p.grad = torch.zeros(9000)
+        opt.step()
+        opt.state[p] = {**opt.state[p], k: opt.state[p][k].to("meta")}
+        n = len(stubbed_adamw)
+        for use in (opt.step, opt.moments):
+            with pytest.raises(_lib.BtsAdmError):
+                use()
+        assert len(stubbed_adamw) == n
