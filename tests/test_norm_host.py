@@ -597,6 +597,6 @@ def test_adamw_refuses_states_on_another_device(stubbed_adamw, bits):
         opt.state[p] = {**opt.state[p], k: opt.state[p][k].to("meta")}
         n = len(stubbed_adamw)
         for use in (opt.step, opt.moments):
-            with pytest.raises(_lib.BtsAdmError):
+            with pytest.raises(_lib.BtsAmdError):
                 use()
         assert len(stubbed_adamw) == n
